@@ -65,7 +65,7 @@ enum trf_status {
 
 enum trf_mode { TRF_MODE_TIME = 0, TRF_MODE_FREQ = 1 };
 
-enum trf_dtype { TRF_F32 = 0, TRF_BF16 = 1 };
+enum trf_dtype { TRF_F32 = 0, TRF_BF16 = 1, TRF_F16 = 2 };
 
 /* Arithmetic of the feed-forward GEMMs.
  * TRF_PREC_BF16: every GEMM operand is rounded to bf16, as the reference kernels do
@@ -349,6 +349,81 @@ int trf_pack_mask_head(const trf_mask_band_src* bands, const int32_t* dins, int3
  * n_bands and hidden must be those of the packing.  n_frames = 0 does nothing. */
 int trf_mask_head(const float* X, int32_t n_frames, int32_t n_bands, const int32_t* dins, int32_t hidden,
                   const void* packed, int32_t precision, float* mask, trf_stream_t stream);
+
+/* ---------------------------------------------------------------- paged K/V cache
+ * No counterpart in the reference, which has whole chunks.  Attention of new rows over the K and V of a
+ * sequence's earlier ones, for a program that takes its frames as they come (a live stream) or serves many
+ * sequences of different lengths at once.  A request is one sequence: with the model's time attention, one band's
+ * frames.  Its K and V rows lie in pages of page_size positions (16, 32, 64, 128 or 256), named by its row of
+ * table [n_requests][max_pages]: position p is in page table[r][p / page_size].
+ *     K [n_pages][kv_heads][page_size / 16][head_dim / 8][16 positions][8 features]     16-bit (rotated)
+ *     V [n_pages][kv_heads][page_size / 8][head_dim features][8 positions]              16-bit
+ * A slot is a place in the cache, page * page_size + position % page_size.  head_dim is 64 or 128, the dtype
+ * TRF_BF16 or TRF_F16 (q, K, V and the output alike), head h reads K/V head h / (heads / kv_heads).
+ * state [2 + n_requests] is int32: free pages, refused requests, and the requests' lengths; pool [n_pages] has the
+ * free pages in its first state[0] entries.  A new cache has state = [n_pages, 0, 0, ...] and pool = 0, 1, 2, ...
+ *
+ * One step of n_new[r] rows per request, on one stream, with the rows of all requests one after the other:
+ * trf_page_plan, trf_paged_append, trf_paged_attention (starts and lens = state_out + 2 of the plan), and state_out
+ * copied to state.  All lengths are read on the device, so a captured step replays with other lengths.  Everything
+ * the device holds is checked there: lengths, counts, starts, pages and slots out of range read and write nothing
+ * out of bounds. */
+
+/* Deal pages for n_new[r] more rows of each request (negative: 0) and say where they go.
+ * For request r with length len and n new rows: starts[r] is the first of its rows (starts [n_requests + 1], at most
+ * n_rows), row starts[r] + i has position len + i and the slot of that position, and state_out holds its length
+ * len + n.  New pages come from the end of the pool, in the order of requests and positions, and are
+ * entered in table (its other entries are left); state_out[0] is what the pool has left.
+ * A request is refused if its rows end past n_rows, its length would pass max_pages * page_size or the pool has not
+ * the pages for it and for the requests before it: its length stays, its rows get position and slot -1 (and what
+ * attention gives for them means nothing), and state_out[1] counts it.  Rows behind the last request get -1 as well.
+ * At most 8192 requests, n_rows < 2^30; slots, positions [n_rows].  state_out must not overlap state. */
+int trf_page_plan(const int32_t* state, const int32_t* n_new, int32_t n_requests, int32_t n_rows, const int32_t* pool,
+                  int32_t n_pages, int32_t page_size, int32_t* table, int32_t max_pages, int32_t* state_out,
+                  int32_t* starts, int32_t* slots, int32_t* positions, trf_stream_t stream);
+
+/* Give the pages of the requests with done[r] != 0 back: the ceil(len / page_size) first entries of their table
+ * rows go to the pool from entry state[0] on, in the order of requests and positions; state_out holds the new count
+ * of free pages, 0 refused requests and the lengths, 0 for these requests.  table is left as it is. */
+int trf_page_release(const int32_t* state, const uint8_t* done, int32_t n_requests, int32_t* pool, int32_t n_pages,
+                     int32_t page_size, const int32_t* table, int32_t max_pages, int32_t* state_out, trf_stream_t stream);
+
+/* Write rows of k and v [n_rows][kv_heads][head_dim] to their slots of K and V, k rotated as trf_qkv_rope_gemm does
+ * (feature pairs 2i, 2i + 1; rope = [2][rope_len][head_dim / 2] fp32, cos then sin, read at positions[row]; fp32
+ * arithmetic, one rounding).  q (optional, [n_rows][heads][head_dim]) is rotated likewise into q_out (rows of
+ * heads * head_dim), which may be q itself if its rows are that far apart.  Row strides are in elements, multiples
+ * of 8; a row's heads are contiguous.  rope = NULL: no rotation (positions are not read).  A row whose slot is not one
+ * of the cache, or whose position is not one of the table, is left out: nothing of it is written.  Of two rows with the
+ * same slot either may be the one that is kept, value by value. */
+int trf_paged_append(const uint16_t* q, int64_t q_stride, int32_t heads, const uint16_t* k, int64_t k_stride,
+                     const uint16_t* v, int64_t v_stride, int32_t dtype, int32_t n_rows, const int32_t* slots,
+                     const int32_t* positions, const float* rope, int32_t rope_len, uint16_t* K, uint16_t* V,
+                     int32_t n_pages, int32_t page_size, int32_t kv_heads, int32_t head_dim, uint16_t* q_out,
+                     trf_stream_t stream);
+
+/* Workspace bytes of trf_paged_attention for these arguments (0: none is needed, or an argument is out of range). */
+size_t trf_paged_attention_workspace_bytes(int32_t heads, int32_t dtype, int32_t n_pages, int32_t page_size,
+                                           int32_t kv_heads, int32_t head_dim, int32_t max_pages, int32_t n_requests,
+                                           int32_t n_rows, int32_t max_new, int32_t max_len);
+
+/* O [n_rows][heads * head_dim] = gate * softmax(scale * q K^T) V.  Rows starts[r] .. starts[r + 1] - 1 of
+ * q [n_rows][heads][head_dim] (rotated) are the last rows of request r, whose length lens[r] counts them: row i of n
+ * is position p = lens[r] - n + i.  It sees the keys j < lens[r], with causal = 1 those with j <= p, and with window > 0
+ * those with j > p - window; keys whose table entry is no page count as unseen.  A row that sees none is zero, and so
+ * is one whose scores are all minus infinity.  What K and V hold in places that a row does not see, infinities and NaN
+ * included, does not change it.  gate [n_rows][heads] fp32 is optional (NULL: 1).  Rows of O behind the last request
+ * are left as they are.
+ * max_new and max_len are the caller's bounds on the rows and the length of a request, from which the launch is
+ * chosen: rows past max_new may be left out, max_len bounds nothing but speed.  P is rounded to the dtype for P V,
+ * unnormalised; scores, their maximum and the sums are fp32.  The same call gives the same bits.
+ * workspace: trf_paged_attention_workspace_bytes, 16-byte aligned, of any content, in use until the call's work is
+ * done: calls that may overlap need one each. */
+int trf_paged_attention(const uint16_t* q, int64_t q_stride, int32_t heads, const uint16_t* K, const uint16_t* V,
+                        int32_t dtype, int32_t n_pages, int32_t page_size, int32_t kv_heads, int32_t head_dim,
+                        const int32_t* table, int32_t max_pages, const int32_t* starts, const int32_t* lens,
+                        int32_t n_requests, int32_t n_rows, int32_t max_new, int32_t max_len, float scale, int32_t causal,
+                        int32_t window, const float* gate, uint16_t* O, void* workspace, size_t workspace_bytes,
+                        trf_stream_t stream);
 
 #ifdef __cplusplus
 }

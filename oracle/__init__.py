@@ -10,6 +10,7 @@ Modules
     reference  fp32 restatement of the reference module forward (src/turbo_roformer/model.py:28-278)
     folded     the restructured forward with folded norms (src/turbo_roformer/fast.py:163-266, 349-360)
     kernels    bf16-rounding emulations of the reference's fused ops (src/turbo_roformer/csrc/kernels.cpp)
+    paged      the paged K/V cache: pages, rotated rows and attention by their definitions, in 64 bits
     cpu_stack  the AVX512-BF16 CPU stack (cpu_stack.cpp, built by the Makefile here): the same-host
                kernel-class CPU baseline of bench.py, after the reference's published CPU kernel design
                (docs/how-it-works.md:120-151)

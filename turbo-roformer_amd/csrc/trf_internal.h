@@ -198,4 +198,42 @@ void launch_pack_mask_band(const float* w1, const float* gamma, const float* b1,
 void launch_mask_head(const float* X, const uint8_t* packed, float* mask, const MaskPlan& plan, unsigned grid,
                       int precision, hipStream_t st);
 
+// ---------------------------------------------------------------- paged K/V cache (trf_pages.hip, trf_paged_attn.hip)
+// Largest number of requests of a plan or release: their prefix sums are formed in LDS.  62 bands x 132 streams.
+constexpr int kPageRequests = 8192;
+
+struct PagePlan {
+  int32_t n_requests, n_rows, n_pages, page_shift, max_pages;  // page_shift: log2 of the page size
+};
+
+// K [n_pages][kv_heads][page / 16][head_dim / 8][16][8], V [n_pages][kv_heads][page / 8][head_dim][8]: the 16
+// positions of a group are one contiguous run of 32 * head_dim bytes in the order of MFMA A operands, whatever the page.
+struct PagedShape {
+  int32_t n_pages, page_shift, kv_heads, head_dim;
+  bool f16;
+};
+
+void launch_page_plan(const PagePlan& p, const int32_t* state, const int32_t* n_new, const int32_t* pool,
+                      int32_t* table, int32_t* state_out, int32_t* starts, int32_t* slots, int32_t* positions,
+                      hipStream_t st);
+void launch_page_release(const PagePlan& p, const int32_t* state, const uint8_t* done, int32_t* pool,
+                         const int32_t* table, int32_t* state_out, hipStream_t st);
+void launch_paged_append(const PagedShape& s, const uint16_t* q, int64_t q_stride, int heads, const uint16_t* k,
+                         int64_t k_stride, const uint16_t* v, int64_t v_stride, uint16_t* K, uint16_t* V,
+                         const int32_t* slots, const int32_t* positions, int32_t n_rows, const float* rope,
+                         int32_t rope_len, uint16_t* q_out, hipStream_t st);
+
+struct PagedAttnArgs {
+  const uint16_t *q, *K, *V;
+  const int32_t *table, *starts, *lens;
+  const float* gate;
+  uint16_t* o;
+  int64_t q_stride;
+  int32_t n_requests, n_rows, heads, max_pages, max_new, max_len, causal, window;
+  float scale_log2;  // the scores' scale times log2(e)
+};
+
+void launch_paged_attention(const PagedShape& s, const PagedAttnArgs& a, void* workspace, hipStream_t st);
+size_t paged_attention_workspace(const PagedShape& s, const PagedAttnArgs& a);
+
 }  // namespace trf

@@ -1,0 +1,356 @@
+// Pages of the paged K/V cache on gfx950: dealing them to requests, taking them back, and the write of new K and V
+// rows into them (the layouts are in trf_hip.h).
+#include <algorithm>
+
+#include "trf_device.h"
+
+namespace trf {
+
+// ============================================================ prefix sums over the requests
+// Every workgroup of a plan or a release forms the prefix sums over all requests itself: at most kPageRequests of
+// them, read from L2, against a second launch or a wait between workgroups.  Thread t holds requests
+// t * each .. t * each + each - 1.
+constexpr int kPageThreads = 1024;
+static_assert(kPageRequests <= 8 * kPageThreads, "requests per thread");
+
+// Exclusive prefix sum over the workgroup's threads in thread order; `total` is the sum.  Sums saturate at
+// most (every term is at most most <= 2^31 - 1), which is as associative as plain addition of whole numbers.
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t most, uint32_t* lds, uint32_t& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t incl = x;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t y = __shfl_up(incl, d);
+    if (lane >= d) incl = min(incl + y, most);
+  }
+  uint32_t excl = __shfl_up(incl, 1);
+  if (lane == 0) excl = 0;
+  __syncthreads();  // the sums of an earlier call have been read
+  if (lane == 63) lds[wave] = incl;
+  __syncthreads();
+  uint32_t before = 0;
+  total = 0;
+  for (int w = 0; w < kPageThreads / 64; ++w) {
+    if (w == wave) before = total;
+    total = min(total + lds[w], most);
+  }
+  return min(before + excl, most);
+}
+
+// Last index r in [0, n) with a[r] <= v, for ascending a with a[0] <= v.
+__device__ __forceinline__ int last_not_above(const uint32_t* a, int n, uint32_t v) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a[mid] <= v)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int clamped_length(int len, const PagePlan& p) {
+  return min(max(len, 0), p.max_pages << p.page_shift);
+}
+
+// ============================================================ plan
+// One thread per new row: its request by binary search over the row starts in LDS, its page from the request's
+// table row or, past the pages it has, from the pool; the row that opens a new page enters it in the table (a new
+// page's first position is always a new row).  Bound by latency: two prefix sums and one search, a few us.
+__global__ __launch_bounds__(kPageThreads) void k_page_plan(PagePlan p, const int32_t* __restrict__ state,
+                                                            const int32_t* __restrict__ n_new,
+                                                            const int32_t* __restrict__ pool, int32_t* table,
+                                                            int32_t* __restrict__ state_out,
+                                                            int32_t* __restrict__ starts, int32_t* __restrict__ slots,
+                                                            int32_t* __restrict__ positions) {
+  __shared__ uint32_t begin[kPageRequests];  // first row of each request
+  __shared__ int32_t dealt[kPageRequests];   // pages dealt before it, or -1: refused
+  __shared__ uint32_t sums[kPageThreads / 64];
+  __shared__ int32_t counts[2];              // pages dealt, requests refused
+  const int R = p.n_requests, each = (R + kPageThreads - 1) / kPageThreads;
+  const int r0 = threadIdx.x * each, r1 = min(r0 + each, R);
+  const uint32_t beyond = uint32_t(p.n_rows) + 1;  // row sums end here
+  const int page = 1 << p.page_shift;
+  const int free = min(max(state[0], 0), p.n_pages);
+  if (threadIdx.x < 2) counts[threadIdx.x] = 0;
+
+  uint32_t mine = 0;
+  for (int r = r0; r < r1; ++r) mine = min(mine + min(uint32_t(max(n_new[r], 0)), beyond), beyond);
+  uint32_t rows;
+  uint32_t row = block_scan(mine, beyond, sums, rows);
+  uint32_t want_mine = 0;
+  {
+    uint32_t b = row;
+    for (int r = r0; r < r1; ++r) {
+      const uint32_t n = min(uint32_t(max(n_new[r], 0)), beyond);
+      const int len = clamped_length(state[2 + r], p);
+      const bool fits = b + n < beyond && int64_t(len) + n <= int64_t(p.max_pages) << p.page_shift;
+      if (fits) want_mine += (len + n + page - 1) / page - (len + page - 1) / page;
+      begin[r] = b;
+      b = min(b + n, beyond);
+    }
+  }
+  uint32_t wanted;
+  uint32_t before = block_scan(want_mine, 0x7fffffffu, sums, wanted);
+  int used = 0, refused = 0;
+  for (int r = r0; r < r1; ++r) {
+    const uint32_t b = begin[r];
+    const uint32_t n = min(uint32_t(max(n_new[r], 0)), beyond);
+    const int len = clamped_length(state[2 + r], p);
+    const bool fits = b + n < beyond && int64_t(len) + n <= int64_t(p.max_pages) << p.page_shift;
+    const uint32_t want = fits ? (len + n + page - 1) / page - (len + page - 1) / page : 0;
+    const bool ok = fits && (want == 0 || before + want <= uint32_t(free));
+    dealt[r] = ok ? int32_t(min(before, uint32_t(free))) : -1;
+    if (ok) used += want;
+    refused += !ok && n > 0;
+    if (blockIdx.x == 0) {
+      starts[r] = min(b, uint32_t(p.n_rows));
+      state_out[2 + r] = ok ? len + n : len;
+    }
+    before += want;
+  }
+  if (blockIdx.x == 0) {
+    if (used) atomicAdd(&counts[0], used);
+    if (refused) atomicAdd(&counts[1], refused);
+  }
+  __syncthreads();
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    starts[R] = min(rows, uint32_t(p.n_rows));
+    state_out[0] = free - counts[0];
+    state_out[1] = counts[1];
+  }
+  for (int64_t i = int64_t(blockIdx.x) * kPageThreads + threadIdx.x; i < p.n_rows; i += int64_t(gridDim.x) * kPageThreads) {
+    int pos = -1, slot = -1;
+    if (uint32_t(i) < rows) {
+      const int r = last_not_above(begin, R, uint32_t(i));
+      const int d = dealt[r];
+      if (d >= 0) {
+        const int len = clamped_length(state[2 + r], p);
+        const int have = (len + page - 1) >> p.page_shift;
+        pos = len + int(uint32_t(i) - begin[r]);
+        const int at = pos >> p.page_shift;
+        int32_t* entry = table + int64_t(r) * p.max_pages + at;
+        int pg;
+        if (at < have) {
+          pg = *entry;
+        } else {
+          pg = pool[free - 1 - (d + at - have)];
+          if ((pos & (page - 1)) == 0) *entry = pg;
+        }
+        if (uint32_t(pg) < uint32_t(p.n_pages)) slot = (pg << p.page_shift) + (pos & (page - 1));
+      }
+    }
+    slots[i] = slot;
+    positions[i] = pos;
+  }
+}
+
+void launch_page_plan(const PagePlan& p, const int32_t* state, const int32_t* n_new, const int32_t* pool,
+                      int32_t* table, int32_t* state_out, int32_t* starts, int32_t* slots, int32_t* positions,
+                      hipStream_t st) {
+  const unsigned grid = unsigned(std::min<int64_t>(std::max<int64_t>((int64_t(p.n_rows) + 2 * kPageThreads - 1) / (2 * kPageThreads), 1), 256));
+  k_page_plan<<<grid, kPageThreads, 0, st>>>(p, state, n_new, pool, table, state_out, starts, slots, positions);
+}
+
+// ============================================================ release
+// One thread per released page: its request by binary search over the prefix sums in LDS.
+__global__ __launch_bounds__(kPageThreads) void k_page_release(PagePlan p, const int32_t* __restrict__ state,
+                                                               const uint8_t* __restrict__ done,
+                                                               int32_t* __restrict__ pool,
+                                                               const int32_t* __restrict__ table,
+                                                               int32_t* __restrict__ state_out) {
+  __shared__ uint32_t before[kPageRequests];  // pages released before the request's
+  __shared__ uint32_t sums[kPageThreads / 64];
+  const int R = p.n_requests, each = (R + kPageThreads - 1) / kPageThreads;
+  const int r0 = threadIdx.x * each, r1 = min(r0 + each, R);
+  const int page = 1 << p.page_shift;
+  const int free = min(max(state[0], 0), p.n_pages);
+  auto pages_of = [&](int r) {
+    return done[r] ? uint32_t(clamped_length(state[2 + r], p) + page - 1) >> p.page_shift : 0u;
+  };
+  uint32_t mine = 0;
+  for (int r = r0; r < r1; ++r) mine += pages_of(r);
+  uint32_t total;
+  uint32_t at = block_scan(mine, 0x7fffffffu, sums, total);
+  for (int r = r0; r < r1; ++r) {
+    before[r] = at;
+    at += pages_of(r);
+    if (blockIdx.x == 0) state_out[2 + r] = done[r] ? 0 : clamped_length(state[2 + r], p);
+  }
+  const uint32_t room = uint32_t(p.n_pages - free);
+  total = min(total, room);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    state_out[0] = free + int(total);
+    state_out[1] = 0;
+  }
+  __syncthreads();
+  for (uint32_t k = blockIdx.x * kPageThreads + threadIdx.x; k < total; k += gridDim.x * kPageThreads) {
+    const int r = last_not_above(before, R, k);
+    pool[free + k] = table[int64_t(r) * p.max_pages + (k - before[r])];
+  }
+}
+
+void launch_page_release(const PagePlan& p, const int32_t* state, const uint8_t* done, int32_t* pool,
+                         const int32_t* table, int32_t* state_out, hipStream_t st) {
+  const int64_t most = std::min<int64_t>(int64_t(p.n_requests) * p.max_pages, p.n_pages);
+  const unsigned grid = unsigned(std::min<int64_t>((most + 4 * kPageThreads - 1) / (4 * kPageThreads), 128));
+  k_page_release<<<std::max(grid, 1u), kPageThreads, 0, st>>>(p, state, done, pool, table, state_out);
+}
+
+// ============================================================ append
+// Rows of k, v (and q) into the cache.  K keeps a position's 16-byte feature chunks 256 bytes apart and the
+// chunks of 16 positions side by side: a wave takes 16 rows and 4 chunks, holds their angles and goes through
+// the heads.  V keeps the 8 positions of an octet side by side per feature: a wave takes the rows of one octet,
+// turns them in LDS and stores 16 bytes a feature, or single values where the call does not fill the octet.
+// Bound by HBM for many rows.
+struct AppendArgs {
+  const uint16_t *q, *k, *v;
+  int64_t q_stride, k_stride, v_stride;  // elements from row to row
+  int32_t heads, kv_heads, n_rows, rope_len, slots, page_shift;
+  const int32_t *slot, *position;
+  const float* rope;
+  uint16_t *q_out, *K, *V;
+  int32_t heads_per, qk_blocks, rows_per;
+};
+
+// Whether row i is written: a slot of the cache and, with a table, one of its positions.
+__device__ __forceinline__ bool live_row(const AppendArgs& a, int i, int& slot) {
+  slot = a.slot[i];
+  return uint32_t(slot) < uint32_t(a.slots) && (!a.rope || uint32_t(a.position[i]) < uint32_t(a.rope_len));
+}
+
+template <bool F16>
+__device__ __forceinline__ u32x4 turn8(u32x4 x, const f32x4& c, const f32x4& s) {
+  u32x4 y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = x[i];  // a bit_cast of the vector's element itself takes element 0
+    float a, b;
+    if constexpr (F16) {
+      const f16x2 v = __builtin_bit_cast(f16x2, w);
+      a = float(v[0]), b = float(v[1]);
+    } else {
+      a = __uint_as_float(w << 16), b = __uint_as_float(w & 0xffff0000u);
+    }
+    const float ya = a * c[i] - b * s[i], yb = a * s[i] + b * c[i];
+    y[i] = F16 ? pk_f16(ya, yb) : pk_bf16(ya, yb);
+  }
+  return y;
+}
+
+template <int D, bool F16>
+__device__ __forceinline__ void append_qk(const AppendArgs& a, int block, int lane, int wave) {
+  constexpr int kParts = D / 32;                 // waves of 4 chunks that share the rows
+  constexpr int kRowTiles = 4 / kParts;          // 16-row tiles per workgroup
+  const int parts_heads = (a.heads + a.kv_heads + a.heads_per - 1) / a.heads_per;
+  const int hb = block % parts_heads, tile = (block / parts_heads) * kRowTiles + wave / kParts;
+  const int i = tile * 16 + (lane & 15), c = 4 * (wave % kParts) + (lane >> 4);
+  if (i >= a.n_rows) return;
+  int slot;
+  if (!live_row(a, i, slot)) return;
+  f32x4 cs{1.f, 1.f, 1.f, 1.f}, sn{0.f, 0.f, 0.f, 0.f};
+  if (a.rope) {
+    const float* t = a.rope + int64_t(a.position[i]) * (D / 2) + 4 * c;
+    cs = *reinterpret_cast<const f32x4*>(t);
+    sn = *reinterpret_cast<const f32x4*>(t + int64_t(a.rope_len) * (D / 2));
+  }
+  const int gpp_shift = a.page_shift - 4;
+  const int page = slot >> a.page_shift, in = slot & ((1 << a.page_shift) - 1);
+  uint16_t* Kp = a.K + (((int64_t(page) * a.kv_heads << gpp_shift) + (in >> 4)) * 16 * D + c * 128 + (in & 15) * 8);
+  const int h1 = min((hb + 1) * a.heads_per, a.heads + a.kv_heads);
+  for (int h = hb * a.heads_per; h < h1; ++h) {
+    const bool is_q = h < a.heads;
+    const uint16_t* src = is_q ? a.q + i * a.q_stride + h * D : a.k + i * a.k_stride + (h - a.heads) * D;
+    uint16_t* dst = is_q ? a.q_out + (int64_t(i) * a.heads + h) * D + 8 * c
+                         : Kp + ((int64_t(h - a.heads) << gpp_shift) * 16 * D);
+    u32x4 x = *reinterpret_cast<const u32x4*>(src + 8 * c);
+    if (a.rope) x = turn8<F16>(x, cs, sn);
+    *reinterpret_cast<u32x4*>(dst) = x;
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void append_v(const AppendArgs& a, int block, int lane, int wave, uint16_t* lds) {
+  constexpr int kLoads = D / 64;  // 16-byte loads per lane for 8 rows of a head
+  const int first = (block * 4 + wave) * a.rows_per;
+  const int gpp2_shift = a.page_shift - 3;
+  for (int i = first; i < min(first + a.rows_per, a.n_rows); ++i) {
+    int slot, prev;
+    if (!live_row(a, i, slot)) continue;
+    // a row that continues the octet of the row before it is written with that row
+    if ((slot & 7) && i > 0 && live_row(a, i - 1, prev) && prev == slot - 1) continue;
+    const int k8 = lane & 7;
+    int at = -1;
+    const bool in_run = k8 < 8 - (slot & 7) && i + k8 < a.n_rows && live_row(a, i + k8, at) && at == slot + k8;
+    const int run = __builtin_ctzll(~(__ballot(in_run) & 0xffull));
+    const int page = slot >> a.page_shift, in = slot & ((1 << a.page_shift) - 1);
+    uint16_t* Vp = a.V + ((int64_t(page) * a.kv_heads << gpp2_shift) + (in >> 3)) * 8 * D;
+    for (int h = 0; h < a.kv_heads; ++h) {
+      const int row = lane >> 3;
+#pragma unroll
+      for (int l = 0; l < kLoads; ++l) {
+        u32x4 x = zero4();
+        if (row < run)
+          x = *reinterpret_cast<const u32x4*>(a.v + (i + row) * a.v_stride + h * D + 64 * l + 8 * (lane & 7));
+        *reinterpret_cast<u32x4*>(lds + row * D + 64 * l + 8 * (lane & 7)) = x;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      uint16_t* dst = Vp + (int64_t(h) << gpp2_shift) * 8 * D;
+#pragma unroll
+      for (int l = 0; l < kLoads; ++l) {
+        const int d = 64 * l + lane;
+        uint16_t e[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) e[k] = lds[k * D + d];
+        if (run == 8) {
+          u32x4 y;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) y[k] = uint32_t(e[2 * k]) | uint32_t(e[2 * k + 1]) << 16;
+          *reinterpret_cast<u32x4*>(dst + d * 8) = y;
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (k < run) dst[d * 8 + (slot & 7) + k] = e[k];
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+}
+
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
+  __shared__ u32x4 lds[4][D];  // 8 rows of D values a wave
+  const int lane = threadIdx.x & 63, wave = wave_id();
+  if (int(blockIdx.x) < a.qk_blocks)
+    append_qk<D, F16>(a, blockIdx.x, lane, wave);
+  else
+    append_v<D>(a, blockIdx.x - a.qk_blocks, lane, wave, reinterpret_cast<uint16_t*>(lds[wave]));
+}
+
+void launch_paged_append(const PagedShape& s, const uint16_t* q, int64_t q_stride, int heads, const uint16_t* k,
+                         int64_t k_stride, const uint16_t* v, int64_t v_stride, uint16_t* K, uint16_t* V,
+                         const int32_t* slots, const int32_t* positions, int32_t n_rows, const float* rope,
+                         int32_t rope_len, uint16_t* q_out, hipStream_t st) {
+  AppendArgs a{};
+  a.q = q, a.k = k, a.v = v;
+  a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride;
+  a.heads = q ? heads : 0, a.kv_heads = s.kv_heads, a.n_rows = n_rows, a.rope_len = rope_len;
+  a.slots = s.n_pages << s.page_shift, a.page_shift = s.page_shift;
+  a.slot = slots, a.position = positions, a.rope = rope;
+  a.q_out = q_out, a.K = K, a.V = V;
+  a.heads_per = 4;
+  a.rows_per = n_rows > 16384 ? 8 : 1;
+  const int rows = 16 * (4 / (s.head_dim / 32));
+  const int parts = (a.heads + a.kv_heads + a.heads_per - 1) / a.heads_per;
+  a.qk_blocks = (n_rows + rows - 1) / rows * parts;
+  const unsigned grid = a.qk_blocks + (n_rows + 4 * a.rows_per - 1) / (4 * a.rows_per);
+  auto kernel = s.head_dim == 64 ? (s.f16 ? k_paged_append<64, true> : k_paged_append<64, false>)
+                                 : (s.f16 ? k_paged_append<128, true> : k_paged_append<128, false>);
+  kernel<<<grid, 256, 0, st>>>(a);
+}
+
+}  // namespace trf

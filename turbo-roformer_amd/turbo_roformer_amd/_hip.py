@@ -30,7 +30,8 @@ PREC_BF16, PREC_FF_SPLIT, PREC_FF_FP16 = 0, 1, 2
 PRECISIONS = {"bf16": PREC_BF16, "ff_split": PREC_FF_SPLIT, "ff_fp16": PREC_FF_FP16}
 MASK_SPLIT, MASK_FP16 = 0, 1
 MASK_PRECISIONS = {"split": MASK_SPLIT, "fp16": MASK_FP16}
-_F32, _BF16 = 0, 1
+_F32, _BF16, _F16 = 0, 1, 2
+_CACHE_DTYPES = {torch.bfloat16: _BF16, torch.float16: _F16}
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
@@ -113,6 +114,18 @@ _SIGNATURES: dict[str, tuple] = {
         ctypes.c_int, [ctypes.POINTER(TrfMaskBandSrc), ctypes.POINTER(ctypes.c_int32), _I32, _I32, _P, _P, _P]
     ),
     "trf_mask_head": (ctypes.c_int, [_P, _I32, _I32, ctypes.POINTER(ctypes.c_int32), _I32, _P, _I32, _P, _P]),
+    "trf_page_plan": (ctypes.c_int, [_P, _P, _I32, _I32, _P, _I32, _I32, _P, _I32, _P, _P, _P, _P, _P]),
+    "trf_page_release": (ctypes.c_int, [_P, _P, _I32, _P, _I32, _I32, _P, _I32, _P, _P]),
+    "trf_paged_append": (
+        ctypes.c_int,
+        [_P, _I64, _I32, _P, _I64, _P, _I64, _I32, _I32, _P, _P, _P, _I32, _P, _P, _I32, _I32, _I32, _I32, _P, _P],
+    ),
+    "trf_paged_attention_workspace_bytes": (_SZ, [_I32] * 11),
+    "trf_paged_attention": (
+        ctypes.c_int,
+        [_P, _I64, _I32, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _I32, _P, _P, _I32, _I32, _I32, _I32, _F, _I32, _I32, _P,
+         _P, _P, _SZ, _P],
+    ),
 }
 
 
@@ -625,3 +638,161 @@ def overlap_finish(acc: torch.Tensor, wsum: torch.Tensor, gain: float, out: torc
     _need(wsum, "wsum", torch.float32, (n,))
     _need(out, "out", torch.float32, (2, n))
     _check(lib.trf_overlap_finish(acc.data_ptr(), wsum.data_ptr(), n, float(gain), out.data_ptr(), _stream()))
+
+
+# ---------------------------------------------------------------------------------------------- paged K/V cache
+
+
+def _ints(t: torch.Tensor, name: str, shape: tuple) -> int:
+    """The address of a contiguous int32 tensor of this shape on the current device."""
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, heads: int, dim: int) -> int:
+    """The row stride, in elements, of rows t [n, heads, dim] whose heads are contiguous (a slice of a projection's
+    rows is)."""
+    if t.dtype != dtype or t.dim() != 3 or t.shape != (n, heads, dim):
+        raise ValueError(f"{name} must be {dtype} {(n, heads, dim)}, got {t.dtype} {tuple(t.shape)}")
+    row, head, one = t.stride()
+    if one != 1 or (heads > 1 and head != dim):
+        raise ValueError(f"{name}'s heads must be contiguous in a row, got strides {t.stride()}")
+    return row if n > 1 else heads * dim
+
+
+def _here(*tensors: torch.Tensor | None) -> None:
+    """All of them are on the current device, whose current stream the call is enqueued on."""
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise ValueError(f"the tensors must be on the current device, cuda:{here}, got one on {t.device}")
+
+
+def _cache(K: torch.Tensor, V: torch.Tensor) -> tuple[int, int, int, int, int]:
+    """(dtype code, pages, page size, K/V heads, head dim) of a paged cache."""
+    if K.dim() != 6 or K.shape[4] != 16 or K.shape[5] != 8 or K.dtype not in _CACHE_DTYPES or not K.is_contiguous():
+        raise ValueError("K must be contiguous bfloat16 or float16 [pages, kv heads, page size / 16, head dim / 8, 16, 8], "
+                         f"got {K.dtype} {tuple(K.shape)}")
+    pages, heads, groups, chunks = K.shape[:4]
+    if V.shape != (pages, heads, 2 * groups, 8 * chunks, 8) or V.dtype != K.dtype or not V.is_contiguous():
+        raise ValueError(f"V must be contiguous {K.dtype} {(pages, heads, 2 * groups, 8 * chunks, 8)}, got {V.dtype} "
+                         f"{tuple(V.shape)}")
+    return _CACHE_DTYPES[K.dtype], pages, 16 * groups, heads, 8 * chunks
+
+
+def paged_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
+                device="cuda") -> tuple[torch.Tensor, torch.Tensor]:
+    """K [pages, kv heads, page size / 16, head dim / 8, 16, 8] and V [pages, kv heads, page size / 8, head dim, 8] of a
+    paged cache (trf_hip.h), not initialised."""
+    if page_size not in (16, 32, 64, 128, 256):
+        raise ValueError(f"page_size must be 16, 32, 64, 128 or 256, got {page_size}")
+    if head_dim not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, got {head_dim}")
+    if dtype not in _CACHE_DTYPES:
+        raise ValueError(f"dtype must be bfloat16 or float16, got {dtype}")
+    K = torch.empty(pages, kv_heads, page_size // 16, head_dim // 8, 16, 8, dtype=dtype, device=device)
+    V = torch.empty(pages, kv_heads, page_size // 8, head_dim, 8, dtype=dtype, device=device)
+    return K, V
+
+
+def page_plan(state, n_new, pool, table, page_size: int, state_out, starts, slots, positions) -> None:
+    """Deal pages for ``n_new`` [R] more rows of each request and say where they go (``trf_page_plan``): ``state`` [2 + R]
+    (free pages, refused requests, lengths) -> ``state_out``, ``table`` [R, max pages] in place, ``starts`` [R + 1],
+    and for each of the rows that ``slots`` and ``positions`` have room for its slot and position, -1 where there
+    is none.  All int32 on the device."""
+    lib = load()
+    R, max_pages = table.shape
+    n = slots.shape[0]
+    _here(state, n_new, pool, table, state_out, starts, slots, positions)
+    _check(lib.trf_page_plan(_ints(state, "state", (2 + R,)), _ints(n_new, "n_new", (R,)), R, n,
+                             _ints(pool, "pool", pool.shape[:1]), pool.shape[0], page_size,
+                             _ints(table, "table", (R, max_pages)), max_pages, _ints(state_out, "state_out", (2 + R,)),
+                             _ints(starts, "starts", (R + 1,)), _ints(slots, "slots", (n,)),
+                             _ints(positions, "positions", (n,)), _stream()))
+
+
+def page_release(state, done, pool, table, page_size: int, state_out) -> None:
+    """Give the pages of the requests with ``done`` [R] (bool or uint8) back to ``pool``, in place
+    (``trf_page_release``): ``state`` [2 + R] -> ``state_out``, their lengths 0."""
+    lib = load()
+    R, max_pages = table.shape
+    _here(state, done, pool, table, state_out)
+    if done.dtype not in (torch.bool, torch.uint8) or done.shape != (R,) or not done.is_contiguous():
+        raise ValueError(f"done must be contiguous bool or uint8 ({R},), got {done.dtype} {tuple(done.shape)}")
+    _check(lib.trf_page_release(_ints(state, "state", (2 + R,)), done.data_ptr(), R, _ints(pool, "pool", pool.shape[:1]),
+                                pool.shape[0], page_size, _ints(table, "table", (R, max_pages)), max_pages,
+                                _ints(state_out, "state_out", (2 + R,)), _stream()))
+
+
+def paged_append(k, v, K, V, slots, positions=None, rope=None, q=None, q_out=None) -> None:
+    """Write rows ``k``, ``v`` [n, kv heads, head dim] (any row stride) to their ``slots`` [n] of the cache ``K``, ``V``, k
+    rotated at ``positions`` [n] by the fp32 table ``rope`` [2, P, head dim / 2] (None: as it is), and ``q`` [n, heads, head
+    dim] rotated likewise into ``q_out`` (``trf_paged_append``).  Rows without a slot (-1) are left out."""
+    lib = load()
+    code, pages, page_size, kv, dim = _cache(K, V)
+    n = k.shape[0]
+    _here(k, v, K, V, slots, positions, rope, q, q_out)
+    ks, vs = _rows(k, "k", K.dtype, n, kv, dim), _rows(v, "v", K.dtype, n, kv, dim)
+    heads = qs = P = 0
+    if rope is not None:
+        P = rope.shape[1] if rope.dim() == 3 else 0
+        if rope.dtype != torch.float32 or rope.shape != (2, P, dim // 2) or not rope.is_contiguous():
+            raise ValueError(f"rope must be contiguous float32 (2, P, {dim // 2}), got {rope.dtype} {tuple(rope.shape)}")
+        if positions is None:
+            raise ValueError("a rotation needs positions")
+    if q is not None:
+        if q.dim() != 3 or q_out is None:
+            raise ValueError("q must be [n, heads, head dim], with a q_out")
+        heads = q.shape[1]
+        qs = _rows(q, "q", K.dtype, n, heads, dim)
+        _need(q_out, "q_out", K.dtype, (n, heads, dim))
+    _check(lib.trf_paged_append(_ptr(q), qs, heads, k.data_ptr(), ks, v.data_ptr(), vs, code, n, _ints(slots, "slots", (n,)),
+                                None if positions is None else _ints(positions, "positions", (n,)), _ptr(rope), P,
+                                K.data_ptr(), V.data_ptr(), pages, page_size, kv, dim, _ptr(q_out), _stream()))
+
+
+def paged_attention(q, K, V, table, starts, lens, O, scale: float | None = None, causal: bool = True, window: int = 0,
+                    gate=None, max_new: int | None = None, max_len: int | None = None, ws=None) -> None:
+    """O [n, heads * head dim] = gate * softmax(scale q K^T) V of the new rows q [n, heads, head dim] over their requests'
+    positions in the paged cache (``trf_paged_attention``).  Rows ``starts[r]`` .. ``starts[r + 1] - 1`` are the last ones
+    of request r, whose length ``lens[r]`` counts them.
+
+    ``scale``: None is head_dim ** -0.5; ``causal``: a row sees no later position; ``window`` > 0: only that many, up to
+    its own; ``gate`` [n, heads] fp32.  ``max_new``, ``max_len``: bounds on the rows and the length of a request (None:
+    n, and what a table row holds): the tighter, the better the launch fits.  ``ws``: uint8 workspace of
+    ``paged_attention_workspace_bytes`` (None: one from torch's allocator for this call)."""
+    lib = load()
+    code, pages, page_size, kv, dim = _cache(K, V)
+    R, max_pages = table.shape
+    if q.dim() != 3:
+        raise ValueError(f"q must be [n, heads, head dim], got {tuple(q.shape)}")
+    n, heads = q.shape[:2]
+    _here(q, K, V, table, starts, lens, O, gate, ws)
+    qs = _rows(q, "q", K.dtype, n, heads, dim)
+    if O.dtype != K.dtype or O.shape != (n, heads * dim) or not O.is_contiguous():
+        raise ValueError(f"O must be contiguous {K.dtype} {(n, heads * dim)}, got {O.dtype} {tuple(O.shape)}")
+    if gate is not None:
+        _need(gate, "gate", torch.float32, (n, heads))
+    if max_new is None:
+        max_new = n
+    if max_len is None:
+        max_len = max_pages * page_size
+    shape = (heads, code, pages, page_size, kv, dim)
+    need = lib.trf_paged_attention_workspace_bytes(*shape, max_pages, R, n, max_new, max_len)
+    if ws is not None:
+        _need(ws, "ws", torch.uint8)
+    elif need:
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _check(lib.trf_paged_attention(q.data_ptr(), qs, heads, K.data_ptr(), V.data_ptr(), *shape[1:],
+                                   _ints(table, "table", (R, max_pages)), max_pages, _ints(starts, "starts", (R + 1,)),
+                                   _ints(lens, "lens", (R,)), R, n, max_new, max_len,
+                                   dim**-0.5 if scale is None else scale, int(causal), window, _ptr(gate), O.data_ptr(),
+                                   _ptr(ws), 0 if ws is None else ws.numel(), _stream()))
+
+
+def paged_attention_workspace_bytes(heads: int, K: torch.Tensor, V: torch.Tensor, n_requests: int, max_pages: int,
+                                    n_rows: int, max_new: int, max_len: int) -> int:
+    """Bytes of the workspace of ``paged_attention`` for these sizes (0: none)."""
+    return int(load().trf_paged_attention_workspace_bytes(heads, *_cache(K, V), max_pages, n_requests, n_rows, max_new,
+                                                          max_len))
