@@ -365,6 +365,26 @@ def test_unseen_infinities_and_nan_change_nothing(hip, dtype, lens, new, page):
         assert bool(got.isfinite().any())
 
 
+@pytest.mark.parametrize("lens,new", [([90], [1]), ([90], [60]), ([2000], [1])])
+def test_seen_nan_and_infinities_come_out(hip, lens, new):
+    """A NaN in q, in a key's K or an infinite score make NaN of the rows that have them, and of no other."""
+    c = _attn_case(lens, new, 2, 2, 64, 16, BF, 13)
+    c["q"][0, 0, 5] = float("nan")
+    got = _run_attn(c, max_new=max(new))
+    assert bool(got[0, 0].isnan().all()) and not bool(got[0, 1].isnan().any()) and not bool(got[1:].isnan().any())
+    for value in (float("nan"), float("inf")):
+        c = _attn_case(lens, new, 2, 2, 64, 16, BF, 13)
+        c["q"][:] = c["q"].abs() + 0.1
+        k = paged.k_rows(c["K"]).clone()
+        at = lens[0] - 1 - new[0] // 2
+        k[int(c["table"][0, at // 16]) * 16 + at % 16, 1, 7] = value
+        P = c["K"].shape[0]
+        c["K"] = k.view(P, 1, 16, 2, 8, 8).permute(0, 3, 1, 4, 2, 5).contiguous()
+        got = _run_attn(c, max_new=max(new))
+        sees = torch.arange(lens[0] - new[0], lens[0]) >= at
+        assert bool(got[sees, 1].isnan().all()) and bool(got[~sees, 1].isfinite().all()) and bool(got[:, 0].isfinite().all())
+
+
 @pytest.mark.parametrize("D,dtype", [(64, BF), (128, HF)])
 def test_attention_scores_that_rise_late(hip, D, dtype):
     """Keys whose scores stand tens and hundreds above all earlier ones, late in a long sequence and one after the other."""

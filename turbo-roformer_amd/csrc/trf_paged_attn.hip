@@ -126,7 +126,9 @@ __device__ __forceinline__ bool find_tile(const Args& g, int tile, int h, int wi
 template <int D>
 struct Acc {
   f32x16 o[D / 32];
-  float m, l;  // m in the scores' own units; l is this half-wave's part of the sum
+  float m, shift;  // running maximum in the scores' own units, and times the scale (0 while there is none)
+  float limit;     // scores above this raise it: kRaise past it, in the scores' own units
+  f32x4 sum;       // sums of P: column j < 16 in register 0 of lane j, column j + 16 in register 1 (row_sum)
 };
 
 template <int D>
@@ -134,7 +136,9 @@ __device__ __forceinline__ void clear(Acc<D>& s) {
 #pragma unroll
   for (int d = 0; d < D / 32; ++d) s.o[d] = zero16();
   s.m = -INFINITY;
-  s.l = 0.f;
+  s.limit = -INFINITY;
+  s.shift = 0.f;
+  s.sum = f32x4{0.f, 0.f, 0.f, 0.f};
 }
 
 // The keys that a column sees: lo .. lo + n - 1.
@@ -150,42 +154,72 @@ __device__ __forceinline__ Mask mask_of(const Args& g, const Tile& t, int col) {
   return Mask{lo, uint32_t(max(hi - lo, 0))};
 }
 
-// Scores -> P as two B operands; raises m, with o and l, where a score is far above it.
-template <int D, bool F16>
-__device__ __forceinline__ void softmax_tile(const f32x16& s, float c, Acc<D>& acc, u32x4& p0, u32x4& p1) {
+// The sum of the rounded P, the weights that P.V applies, on the matrix pipe instead of by 16 additions a lane:
+// v_mfma_f32_16x16x32 takes P's registers as its B operand, whose lane l is column l % 16 and k-group l / 16; they hold
+// column l % 32 = l % 16 + 16 ((l / 16) & 1).  A's row 0 is 1 on k-groups 0 and 2, row 1 on 1 and 3, the rest 0.
+template <bool F16>
+__device__ __forceinline__ u32x4 sum_rows(int lane) {
+  const int m = lane & 15, k = (lane >> 4) & 1;
+  const uint32_t one = m == k && m < 2 ? (F16 ? 0x3c003c00u : 0x3f803f80u) : 0u;
+  return u32x4{one, one, one, one};
+}
+
+template <bool F16>
+__device__ __forceinline__ f32x4 row_sum(u32x4 ones, u32x4 p, f32x4 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, ones), __builtin_bit_cast(f16x8, p), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ones), __builtin_bit_cast(bf16x8, p), c, 0,
+                                                   0, 0);
+}
+
+// Column j's sum, j = lane % 32 (both halves get it).
+__device__ __forceinline__ float sum_of(const f32x4& sum, int j) {
+  const float a = __shfl(sum[0], j & 15), b = __shfl(sum[1], j & 15);
+  return j < 16 ? a : b;
+}
+
+// The largest score of this lane's half of a column.
+__device__ __forceinline__ float half_max(const f32x16& s) {
   float top = s[0];
 #pragma unroll
   for (int r = 1; r < 15; r += 2) top = fmaxf(fmaxf(top, s[r]), s[r + 1]);
-  top = halfwave_max(fmaxf(top, s[15]));
-  const bool raise = top > acc.m && (top - acc.m) * c > (acc.m == -INFINITY ? 0.f : kRaise);
-  if (__any(raise)) {
-    const float m = raise ? top : acc.m;
-    const float f = raise ? __builtin_amdgcn_exp2f((acc.m - m) * c) : 1.f;
-    acc.m = m;
-    acc.l *= f;
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc.o[d][r] *= f;
-  }
-  const float shift = acc.m == -INFINITY ? 0.f : acc.m * c;
-  float e[16];
-#pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -shift));
-    acc.l += e[r];
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    p0[i] = pack2<F16>(e[2 * i], e[2 * i + 1]);
-    p1[i] = pack2<F16>(e[8 + 2 * i], e[8 + 2 * i + 1]);
-  }
+  return fmaxf(top, s[15]);
 }
 
-// Sum of the halves of a column.
-__device__ __forceinline__ float halfwave_sum(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+// Whether any column of the wave has a score far above its maximum, or its first.
+template <int D>
+__device__ __forceinline__ bool above(const Acc<D>& acc, float top) {
+  return __builtin_amdgcn_ballot_w64(top > acc.limit) != 0;
+}
+
+// Raises the maxima of the columns that are.
+template <int D>
+__device__ __forceinline__ void raise(Acc<D>& acc, float half_top, float c) {
+  const float top = halfwave_max(half_top);
+  const bool up = top > acc.limit;
+  const float f = up ? __builtin_amdgcn_exp2f((acc.m - top) * c) : 1.f;
+  if (up) {
+    acc.m = top;
+    acc.shift = top * c;
+    acc.limit = top + kRaise / c;
+  }
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc.o[d][r] *= f;
+  acc.sum[0] *= f;
+  acc.sum[1] *= __shfl(f, (__lane_id() & 15) + 16);
+}
+
+// Scores -> P as two B operands.
+template <bool F16>
+__device__ __forceinline__ void weights(const f32x16& s, float c, float shift, u32x4& p0, u32x4& p1) {
+  float e[16];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -shift));
+  p0 = u32x4{pack2<F16>(e[0], e[1]), pack2<F16>(e[2], e[3]), pack2<F16>(e[4], e[5]), pack2<F16>(e[6], e[7])};
+  p1 = u32x4{pack2<F16>(e[8], e[9]), pack2<F16>(e[10], e[11]), pack2<F16>(e[12], e[13]), pack2<F16>(e[14], e[15])};
 }
 
 __device__ __forceinline__ float value16(uint16_t v, bool f16) {
@@ -226,12 +260,12 @@ __device__ __forceinline__ void load_q(const Args& g, const Tile& t, int col, in
   for (int ks = 0; ks < D / 16; ++ks) qb[ks] = valid ? *reinterpret_cast<const u32x4*>(q + ks * 16) : zero4();
 }
 
-// Columns' rows out: four features of a column, divided by its sum and gated; zeros for a row that saw no key.
+// Columns' rows out: four features of a column, divided by its sum and gated; zeros for a row that saw no key, whose sum
+// is zero (by its bits: a NaN is not).
 template <int D, bool F16>
-__device__ __forceinline__ void store4(const Args& g, int64_t out, int quad, const f32x4& o, float m, float l) {
-  const float f = m > -INFINITY ? (g.a.gate ? g.a.gate[out] : 1.f) / l : 0.f;
-  const u32x2 y = m > -INFINITY ? u32x2{pack2<F16>(o[0] * f, o[1] * f), pack2<F16>(o[2] * f, o[3] * f)} : u32x2{0u, 0u};
-  *reinterpret_cast<u32x2*>(g.a.o + out * D + 4 * quad) = y;
+__device__ __forceinline__ void store4(const Args& g, int64_t out, int quad, const f32x4& o, float l) {
+  const float f = __float_as_uint(l) << 1 ? (g.a.gate ? g.a.gate[out] : 1.f) / l : 0.f;
+  *reinterpret_cast<u32x2*>(g.a.o + out * D + 4 * quad) = u32x2{pack2<F16>(o[0] * f, o[1] * f), pack2<F16>(o[2] * f, o[3] * f)};
 }
 
 // Row of O (times heads, plus the head) that is column col of the tile's request.
@@ -270,6 +304,8 @@ __global__ __launch_bounds__(64 * kWaves) void k_paged_attn_few(Args g) {
   const Mask mask = mask_of(g, t, col);
   Acc<D> acc;
   clear(acc);
+  const u32x4 ones = sum_rows<F16>(lane);
+  const float c = g.a.scale_log2;
   const int32_t* table = g.a.table + int64_t(t.r) * g.a.max_pages;
   const int gpp_mask = (1 << g.gpp_shift) - 1;
   int k0, k1;
@@ -313,8 +349,11 @@ __global__ __launch_bounds__(64 * kWaves) void k_paged_attn_few(Args g) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) va[d][u][i] = finite2<F16>(va[d][u][i], odd);
     }
+    const float top = half_max(s);
+    if (above(acc, top)) raise(acc, top, c);
     u32x4 p0, p1;
-    softmax_tile<D, F16>(s, g.a.scale_log2, acc, p0, p1);
+    weights<F16>(s, c, acc.shift, p0, p1);
+    acc.sum = row_sum<F16>(ones, p1, row_sum<F16>(ones, p0, acc.sum));
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       acc.o[d] = mfma<F16>(va[d][0], p0, acc.o[d]);
@@ -322,7 +361,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_paged_attn_few(Args g) {
     }
     if (__any(odd)) add_infinities<D, F16>(acc, [&](int u) { return Vg[u]; }, seen, hh);
   }
-  acc.l = halfwave_sum(acc.l);
+  const float l = sum_of(acc.sum, j);
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -331,7 +370,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_paged_attn_few(Args g) {
           f32x4{acc.o[d][4 * q], acc.o[d][4 * q + 1], acc.o[d][4 * q + 2], acc.o[d][4 * q + 3]};
   if (hh == 0) {
     lds_m[wave][j] = acc.m;
-    lds_l[wave][j] = acc.l;
+    lds_l[wave][j] = l;
   }
   __syncthreads();
   for (int x = threadIdx.x; x < kCols * (D / 4); x += 64 * kWaves) {
@@ -341,14 +380,13 @@ __global__ __launch_bounds__(64 * kWaves) void k_paged_attn_few(Args g) {
     for (int w = 0; w < kWaves; ++w) m = fmaxf(m, lds_m[w][cc]);
     f32x4 o{0.f, 0.f, 0.f, 0.f};
     for (int w = 0; w < kWaves; ++w) {
-      if (lds_m[w][cc] == -INFINITY) continue;
-      const float f = __builtin_amdgcn_exp2f((lds_m[w][cc] - m) * g.a.scale_log2);
+      const float f = lds_m[w][cc] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((lds_m[w][cc] - m) * c);
       l += f * lds_l[w][cc];
       o += f * lds_o[w][quad * kQuad + cc];
     }
     const int64_t out = out_row(g, t, t.col0 + cc);
     if (g.splits == 1) {
-      store4<D, F16>(g, out, quad, o, m, l);
+      store4<D, F16>(g, out, quad, o, l);
     } else {
       const int64_t at = int64_t(blockIdx.y) * g.a.n_rows * g.a.heads + out;
       *reinterpret_cast<f32x4*>(g.part_o + at * D + 4 * quad) = o;
@@ -361,159 +399,221 @@ __global__ __launch_bounds__(64 * kWaves) void k_paged_attn_few(Args g) {
 }
 
 // ============================================================ many columns
-// A workgroup has 4 x 32 QT columns, 32 QT a wave.  Tiles of 64 keys stream through a ring of LDS buffers, loaded
-// global->LDS directly: the tile's four 16-key groups lie one after the other, each as the cache has it, and wave w
-// loads group w, of one page.  A wave computes the tiles that its own columns see and meets every barrier.
-template <int D, bool F16, int QT>
-__global__ __launch_bounds__(64 * kWaves, 2) void k_paged_attn_many(Args g) {
+// A workgroup has 4 x 32 columns, 32 a wave.  K and V stream through a ring of LDS buffers, loaded global->LDS directly
+// in stages of 64 (D = 64) or 32 (D = 128) keys: 16-key groups one after the other, each as the cache has it, so that
+// a wave loads one page's part of a stage.
+//
+// A unit is 32 keys.  Matrix and vector work of one unit depend on each other end to end (scores, maximum, P, P.V), so
+// a wave works on three units at once: while P of unit i is formed, the scores of i + 1 and P.V of i - 1 run on the
+// matrix pipe, in the shadow of the exponentials.  Raising the maximum, masks and infinities leave that path (rare).
+template <int D>
+struct Many {
+  static constexpr int kStageKeys = D == 64 ? 64 : 32, kUnits = kStageKeys / 32;  // keys and units of a stage
+  static constexpr int kAhead = D == 64 ? 1 : 2;    // stages whose loads are in flight past the one waited for
+  static constexpr int kBufs = D == 64 ? 3 : 5;     // stages: V of unit i, K of i + 2, and the ones in flight
+  static constexpr int kGroup = 2 * D;              // 16-byte chunks of a 16-key group, K or V
+  static constexpr int kStageGroups = kStageKeys / 16;
+  static constexpr int kStage = 2 * kStageGroups * kGroup;  // chunks of a stage: K groups, then V groups
+  static constexpr int kLoads = kStage / 64 / kWaves;       // 1 KB loads of a wave
+};
+
+template <int D, bool F16>
+__global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void k_paged_attn_many(Args g) {
+  using M = Many<D>;
   constexpr int KS = D / 16, DT = D / 32;
-  constexpr int kGroup = 2 * D;               // 16-byte chunks of a 16-key group, K or V
-  constexpr int kLoads = kGroup / 64;         // 1 KB loads of one
-  constexpr int kWidth = kWaves * kCols * QT;
-  constexpr int kBufs = D == 64 ? 3 : 2;
-  __shared__ u32x4 lds[kBufs][2][4 * kGroup];
+  __shared__ u32x4 lds[M::kBufs][M::kStage];
   const int lane = threadIdx.x & 63, wave = wave_id(), j = lane & 31, hh = lane >> 5;
   Tile t;
-  if (!find_tile(g, blockIdx.x / g.kv_heads, blockIdx.x % g.kv_heads, kWidth, t)) return;
+  if (!find_tile(g, blockIdx.x / g.kv_heads, blockIdx.x % g.kv_heads, kWaves * kCols, t)) return;
   const int32_t* table = g.a.table + int64_t(t.r) * g.a.max_pages;
-  const int gpp_mask = (1 << g.gpp_shift) - 1;
-  int k0, k1;
-  split_range(g, t, 64, k0, k1);
+  const float c = g.a.scale_log2;
+  int s0, s1;  // stages
+  split_range(g, t, M::kStageKeys, s0, s1);
+  const int n_stages = max(s1 - s0, 0), n_units = n_stages * M::kUnits, first_key = s0 * M::kStageKeys;
 
-  // this wave's columns: the keys that any and all of them see
-  const int col0 = t.col0 + wave * kCols * QT, last = min(col0 + kCols * QT, t.cols) - 1;
+  // This wave's share of stage st: part of one group's K or V.
+  constexpr int kParts = M::kLoads * 64 < M::kGroup ? M::kGroup / (M::kLoads * 64) : 1;
+  static_assert(kParts == 1, "a wave loads whole groups");
+  constexpr int kGroupsEach = M::kLoads * 64 / M::kGroup;  // 2: K and V of one 16-key group (D = 64); 1 (D = 128)
+  const int my_group = wave % M::kStageGroups;
+  auto page_of = [&](int st) {
+    return scalar_load(table + min((M::kStageGroups * (s0 + st) + my_group) >> g.gpp_shift, g.a.max_pages - 1));
+  };
+  auto stage = [&](int st, int page) {  // zeros for what is no page
+    const bool ok = uint32_t(page) < uint32_t(g.n_pages);
+    const int in = (M::kStageGroups * (s0 + st) + my_group) & ((1 << g.gpp_shift) - 1);
+    const int64_t at = ((((int64_t(ok ? page : 0) * g.kv_heads + t.h) << g.gpp_shift) + in) * 16) * D;
+    const int bytes = ok ? 32 * D : 0;
+    u32x4* dst = &lds[st % M::kBufs][my_group * M::kGroup];
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      if (kGroupsEach == 1 && v != wave / M::kStageGroups) continue;
+      const __amdgpu_buffer_rsrc_t r = buffer_rsrc((v ? g.a.V : g.a.K) + at, bytes);
+#pragma unroll
+      for (int i = 0; i < M::kGroup / 64; ++i)
+        buffer_load_lds16(r, (64 * i + lane) * 16, dst + v * M::kStageGroups * M::kGroup + 64 * i);
+    }
+  };
+  constexpr int kFirst = 2 / M::kUnits;  // stage that the end of step 0 waits for
+  for (int st = 0; st < min(kFirst + M::kAhead, n_stages); ++st) stage(st, page_of(st));
+  int next = page_of(kFirst + M::kAhead);
+
+  // entries that are no pages: then every unit looks its groups up
+  bool bad = false;
+  const int e1 = min(((t.hi + 15) / 16 + (1 << g.gpp_shift) - 1) >> g.gpp_shift, g.a.max_pages);
+  for (int e = (first_key >> g.page_shift) + lane; e < e1; e += 64) bad |= uint32_t(table[e]) >= uint32_t(g.n_pages);
+  const bool any_bad = __any(bad);
+
+  // this wave's columns, and its units a .. b - 1 (counted from the workgroup's first)
+  const int col0 = t.col0 + wave * kCols, col = col0 + j;
   const bool active = col0 < t.cols;
   int lo = 0, hi = 0, lo_all = 0, hi_all = 0;
-  if (active) key_range(g, t, col0, last, lo, hi, lo_all, hi_all);
+  if (active) key_range(g, t, col0, min(col0 + kCols, t.cols) - 1, lo, hi, lo_all, hi_all);
+  const int a = min(max(lo - first_key, 0) / 32, n_units), b = min((max(hi - first_key, 0) + 31) / 32, n_units);
+  u32x4 qb[KS];
+  load_q<D>(g, t, col, hh, qb);
+  const Mask mask = mask_of(g, t, col);
+  Acc<D> acc;
+  clear(acc);
+  const u32x4 ones = sum_rows<F16>(lane);
 
-  u32x4 qb[QT][KS];
-  Acc<D> acc[QT];
-  Mask mask[QT];
+  // places of units in the ring
+  const int k_lane = (j >> 4) * M::kGroup + hh * 16 + key_slot(j & 15);
+  const int v_lane = M::kStageGroups * M::kGroup + hh * D + j;
+  auto place = [&](int i) { return (i / M::kUnits) % M::kBufs * M::kStage + i % M::kUnits * 2 * M::kGroup; };
+  auto after = [&](int at, int i) {  // unit i's place, after unit i - 1's
+    if (i % M::kUnits) return at + 2 * M::kGroup;
+    at += M::kStage - 2 * M::kGroup * (M::kUnits - 1);
+    return at == M::kBufs * M::kStage ? 0 : at;
+  };
+  // The end of step i, the same for all waves: unit i + 2 lies in LDS, and the next stage's loads are under way.
+  auto advance = [&](int i) {
+    if ((i + 2) % M::kUnits != 0 || i + 2 >= n_units) return;
+    const int st = (i + 2) / M::kUnits;
+    if (M::kAhead > 1 && st + M::kAhead - 1 < n_stages)
+      vmcnt_barrier<M::kLoads*(M::kAhead - 1)>();
+    else
+      vmcnt_barrier<0>();
+    if (st + M::kAhead < n_stages) {
+      stage(st + M::kAhead, next);
+      next = page_of(st + M::kAhead + 1);
+    }
+  };
+  auto group_ok = [&](int key) {  // whether the key's group is in a page, where not all are
+    return !any_bad || uint32_t(scalar_load(table + min(key >> 4 >> g.gpp_shift, g.a.max_pages - 1))) < uint32_t(g.n_pages);
+  };
+
+  // K of unit i + 1, V and P of unit i - 1 (zeros before the first), scores of unit i
+  u32x4 ka[KS], va[DT][2], p0 = zero4(), p1 = zero4();
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    const int col = col0 + kCols * qt + j;
-    load_q<D>(g, t, col, hh, qb[qt]);
-    mask[qt] = mask_of(g, t, col);
-    clear(acc[qt]);
+  for (int d = 0; d < DT; ++d) va[d][0] = va[d][1] = zero4();
+  f32x16 s_even = zero16(), s_odd = zero16();
+  auto load_k = [&](int at) {
+    const u32x4* K = lds[0] + at + k_lane;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) ka[ks] = K[ks * 32];
+  };
+  auto scores = [&](f32x16& s) {
+    s = zero16();
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) s = mfma<F16>(ka[ks], qb[ks], s);
+  };
+  auto p_v = [&]() {
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      acc.o[d] = mfma<F16>(va[d][0], p0, acc.o[d]);
+      acc.o[d] = mfma<F16>(va[d][1], p1, acc.o[d]);
+    }
+  };
+  auto settle = [&]() {  // P.V of the last unit now, and nothing of it later
+    p_v();
+    p0 = p1 = zero4();
+#pragma unroll
+    for (int d = 0; d < DT; ++d) va[d][0] = va[d][1] = zero4();
+  };
+
+  if (n_stages >= kFirst + M::kAhead)
+    vmcnt_barrier<M::kLoads * (kFirst + M::kAhead - 2 / M::kUnits)>();  // units 0 and 1
+  else
+    vmcnt_barrier<0>();
+  for (int i = 0; i < a; ++i) advance(i);
+  if (a < b) {
+    int at = place(a), at1 = after(at, a + 1);
+    load_k(at);
+    scores(s_even);
+    load_k(at1);
+    // units all of whose keys all columns see
+    const int w0 = (max(lo_all - first_key, 0) + 31) / 32, w1 = any_bad ? 0 : max(hi_all - first_key, 0) / 32;
+    auto step = [&](int i, f32x16& s, f32x16& s_next) {
+      const bool whole = i >= w0 && i < w1;
+      const int key0 = first_key + 32 * i;
+      auto seen = [&](int k) { return mask(key0 + k) && group_ok(key0 + (k & 16)); };
+      if (!whole) {
+        const bool ok0 = group_ok(key0), ok1 = group_ok(key0 + 16);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int k = key_in_tile(r, hh);
+          s[r] = mask(key0 + k) && (k < 16 ? ok0 : ok1) ? s[r] : -INFINITY;
+        }
+      }
+      const float top = half_max(s);
+      if (above(acc, top)) {
+        settle();
+        raise(acc, top, c);
+      }
+      scores(s_next);
+      p_v();
+      weights<F16>(s, c, acc.shift, p0, p1);
+      acc.sum = row_sum<F16>(ones, p1, row_sum<F16>(ones, p0, acc.sum));
+      const u32x4* V = lds[0] + at + v_lane;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) va[d][u] = V[u * M::kGroup + 32 * d];
+      if (!whole) {
+        bool odd = false;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) va[d][u][x] = finite2<F16>(va[d][u][x], odd);
+        if (__any(odd)) {
+          settle();
+          const u32x4* unit = lds[0] + at + M::kStageGroups * M::kGroup;
+          add_infinities<D, F16>(acc, [&](int u) { return reinterpret_cast<const uint16_t*>(unit + u * M::kGroup); }, seen, hh);
+        }
+      }
+      advance(i);
+      at = at1;
+      at1 = after(at1, i + 2);
+      load_k(at1);
+    };
+    for (int i = a; i < b; i += 2) {  // two steps a turn: the scores change places without being copied
+      step(i, s_even, s_odd);
+      if (i + 1 < b) step(i + 1, s_odd, s_even);
+    }
+    p_v();
   }
-
-  auto page_of = [&](int kt) {
-    return scalar_load(table + min((4 * kt + wave) >> g.gpp_shift, g.a.max_pages - 1));
-  };
-  auto stage = [&](int kt, int page) {  // this wave's share of tile kt: zeros for what is no page
-    const bool ok = uint32_t(page) < uint32_t(g.n_pages);
-    const int64_t at = ((((int64_t(ok ? page : 0) * g.kv_heads + t.h) << g.gpp_shift) + ((4 * kt + wave) & gpp_mask)) * 16) * D;
-    const int bytes = ok ? 32 * D : 0;
-    const __amdgpu_buffer_rsrc_t Kr = buffer_rsrc(g.a.K + at, bytes), Vr = buffer_rsrc(g.a.V + at, bytes);
-    u32x4* dst = &lds[(kt - k0) % kBufs][0][wave * kGroup];
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      buffer_load_lds16(Kr, (64 * i + lane) * 16, dst + 64 * i);
-      buffer_load_lds16(Vr, (64 * i + lane) * 16, dst + 4 * kGroup + 64 * i);
-    }
-  };
-  // tile kt's operands from LDS, scores, P and P.V, for every column tile
-  auto compute = [&](int kt) {
-    const u32x4* Kl = lds[(kt - k0) % kBufs][0];
-    const u32x4* Vl = lds[(kt - k0) % kBufs][1];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int key0 = 64 * kt + 32 * half;
-      if (key0 >= hi || key0 + 32 <= lo) continue;
-      bool page_ok[2];
-      bool whole = key0 >= lo_all && key0 + 32 <= hi_all;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        page_ok[u] = uint32_t(scalar_load(table + min((4 * kt + 2 * half + u) >> g.gpp_shift, g.a.max_pages - 1))) <
-                     uint32_t(g.n_pages);
-        whole &= page_ok[u];
-      }
-      u32x4 ka[KS];
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        ka[ks] = Kl[(2 * half + (j >> 4)) * kGroup + (2 * ks + hh) * 16 + key_slot(j & 15)];
-      u32x4 p0[QT], p1[QT];
-#pragma unroll
-      for (int qt = 0; qt < QT; ++qt) {
-        f32x16 s = zero16();
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s = mfma<F16>(ka[ks], qb[qt][ks], s);
-        if (!whole) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int k = key_in_tile(r, hh);
-            s[r] = mask[qt](key0 + k) && page_ok[k >> 4] ? s[r] : -INFINITY;
-          }
-        }
-        softmax_tile<D, F16>(s, g.a.scale_log2, acc[qt], p0[qt], p1[qt]);
-      }
-      bool odd = false;
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        u32x4 v[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          v[u] = Vl[(2 * half + u) * kGroup + hh * D + 32 * d + j];
-          if (!whole) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[u][i] = finite2<F16>(v[u][i], odd);
-          }
-        }
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-          acc[qt].o[d] = mfma<F16>(v[0], p0[qt], acc[qt].o[d]);
-          acc[qt].o[d] = mfma<F16>(v[1], p1[qt], acc[qt].o[d]);
-        }
-      }
-      if (__any(odd)) {
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
-          add_infinities<D, F16>(
-              acc[qt], [&](int u) { return reinterpret_cast<const uint16_t*>(Vl + (2 * half + u) * kGroup); },
-              [&](int k) { return mask[qt](key0 + k) && page_ok[k >> 4]; }, hh);
-      }
-    }
-  };
-
-  if (k0 < k1) {
-#pragma unroll
-    for (int i = 0; i < kBufs - 1; ++i)
-      if (k0 + i < k1) stage(k0 + i, page_of(k0 + i));
-    int next = page_of(min(k0 + kBufs - 1, k1));  // page of the tile to be staged next, read a tile ahead
-    for (int kt = k0; kt < k1; ++kt) {
-      if (kBufs > 2 && kt + kBufs - 2 < k1)  // the younger tiles' loads stay in flight
-        vmcnt_barrier<2 * kLoads*(kBufs - 2)>();
-      else
-        vmcnt_barrier<0>();
-      if (kt + kBufs - 1 < k1) {
-        stage(kt + kBufs - 1, next);
-        next = page_of(kt + kBufs);
-      }
-      if (active) compute(kt);
-    }
-  }
+  for (int i = max(a, b); i < n_units; ++i) advance(i);
   if (!active) return;
+  const float l = sum_of(acc.sum, j);
+  if (col >= t.cols) return;
+  const int64_t out = out_row(g, t, col), part = int64_t(blockIdx.y) * g.a.n_rows * g.a.heads + out;
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) {
-    const int col = col0 + kCols * qt + j;
-    const float l = halfwave_sum(acc[qt].l);
-    if (col >= t.cols) continue;
-    const int64_t out = out_row(g, t, col), at = int64_t(blockIdx.y) * g.a.n_rows * g.a.heads + out;
+  for (int d = 0; d < DT; ++d)
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x4 o{acc[qt].o[d][4 * q], acc[qt].o[d][4 * q + 1], acc[qt].o[d][4 * q + 2], acc[qt].o[d][4 * q + 3]};
-        const int quad = 8 * d + 2 * q + hh;
-        if (g.splits == 1)
-          store4<D, F16>(g, out, quad, o, acc[qt].m, l);
-        else
-          *reinterpret_cast<f32x4*>(g.part_o + at * D + 4 * quad) = o;
-      }
-    if (g.splits > 1 && hh == 0) {
-      g.part_ml[2 * at] = acc[qt].m;
-      g.part_ml[2 * at + 1] = l;
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 o{acc.o[d][4 * q], acc.o[d][4 * q + 1], acc.o[d][4 * q + 2], acc.o[d][4 * q + 3]};
+      const int quad = 8 * d + 2 * q + hh;
+      if (g.splits == 1)
+        store4<D, F16>(g, out, quad, o, l);
+      else
+        *reinterpret_cast<f32x4*>(g.part_o + part * D + 4 * quad) = o;
     }
+  if (g.splits > 1 && hh == 0) {
+    g.part_ml[2 * part] = acc.m;
+    g.part_ml[2 * part + 1] = l;
   }
 }
 
@@ -538,7 +638,7 @@ __global__ __launch_bounds__(256) void k_paged_attn_join(Args g, int width) {
       l += f * g.part_ml[2 * at + 1];
       o += f * *reinterpret_cast<const f32x4*>(g.part_o + at * D + 4 * quad);
     }
-    store4<D, F16>(g, out, quad, o, m, l);
+    store4<D, F16>(g, out, quad, o, l);
   }
 }
 
@@ -546,7 +646,7 @@ namespace {
 
 // How a call is run, from what the host knows of it.
 struct Plan {
-  int qt;  // 0: the kernel for few columns; else 32-column tiles per wave of the one for many
+  bool many;  // the kernel for many columns
   int width, tiles, search, splits;
 };
 
@@ -554,13 +654,13 @@ Plan plan_of(const PagedShape& s, const PagedAttnArgs& a) {
   Plan p{};
   const int group = a.heads / s.kv_heads;
   const int64_t most = int64_t(a.max_new) * group;  // columns of a request, at most
-  p.qt = most <= 32 ? 0 : s.head_dim == 128 || most <= kWaves * kCols ? 1 : 2;
-  p.width = p.qt ? kWaves * kCols * p.qt : kCols;
+  p.many = most > 32;
+  p.width = p.many ? kWaves * kCols : kCols;
   p.search = most > p.width;
   p.tiles = p.search ? int(int64_t(a.n_rows) * group / p.width) + a.n_requests : a.n_requests;
   // Parts of the keys: enough workgroups for four on each CU (two of the kernel for many columns), parts of 512 keys
   // at least.
-  const int64_t blocks = int64_t(p.tiles) * s.kv_heads, want = int64_t(device_cu_count()) * (p.qt ? 2 : 4);
+  const int64_t blocks = int64_t(p.tiles) * s.kv_heads, want = int64_t(device_cu_count()) * (p.many ? 2 : 4);
   p.splits = int(std::max<int64_t>(1, std::min<int64_t>({want / blocks, a.max_len / 512, 64})));
   return p;
 }
@@ -575,12 +675,10 @@ size_t paged_attention_workspace(const PagedShape& s, const PagedAttnArgs& a) {
 template <int D, bool F16>
 void launch(const Plan& p, const Args& g, hipStream_t st) {
   const dim3 grid(unsigned(int64_t(p.tiles) * g.kv_heads), unsigned(p.splits));
-  if (p.qt == 0)
+  if (p.many)
+    k_paged_attn_many<D, F16><<<grid, 64 * kWaves, 0, st>>>(g);
+  else
     k_paged_attn_few<D, F16><<<grid, 64 * kWaves, 0, st>>>(g);
-  else if (p.qt == 1)
-    k_paged_attn_many<D, F16, 1><<<grid, 64 * kWaves, 0, st>>>(g);
-  else if constexpr (D == 64)
-    k_paged_attn_many<D, F16, 2><<<grid, 64 * kWaves, 0, st>>>(g);
   if (p.splits > 1) k_paged_attn_join<D, F16><<<grid.x, 256, 0, st>>>(g, p.width);
 }
 
