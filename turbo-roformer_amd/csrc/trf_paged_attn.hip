@@ -11,6 +11,7 @@
 // in 256- and 512-byte runs; key rows go in with bits 2 and 3 of their number swapped, so that the registers of S^T
 // are the B operand of P.V as they stand (key_slot).
 #include <algorithm>
+#include <type_traits>
 
 #include "trf_device.h"
 
@@ -195,7 +196,7 @@ __device__ __forceinline__ bool above(const Acc<D>& acc, float top) {
 
 // Raises the maxima of the columns that are.
 template <int D>
-__device__ __forceinline__ void raise(Acc<D>& acc, float half_top, float c) {
+__device__ __forceinline__ void raise(Acc<D>& acc, float half_top, float c, int lane) {
   const float top = halfwave_max(half_top);
   const bool up = top > acc.limit;
   const float f = up ? __builtin_amdgcn_exp2f((acc.m - top) * c) : 1.f;
@@ -209,17 +210,16 @@ __device__ __forceinline__ void raise(Acc<D>& acc, float half_top, float c) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc.o[d][r] *= f;
   acc.sum[0] *= f;
-  acc.sum[1] *= __shfl(f, (__lane_id() & 15) + 16);
+  acc.sum[1] *= __shfl(f, (lane & 15) + 16);
 }
 
-// Scores -> P as two B operands.
-template <bool F16>
-__device__ __forceinline__ void weights(const f32x16& s, float c, float shift, u32x4& p0, u32x4& p1) {
-  float e[16];
+// Half of a tile's scores -> P as a B operand.
+template <bool F16, int HALF>
+__device__ __forceinline__ u32x4 weights(const f32x16& s, float c, float shift) {
+  float e[8];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -shift));
-  p0 = u32x4{pack2<F16>(e[0], e[1]), pack2<F16>(e[2], e[3]), pack2<F16>(e[4], e[5]), pack2<F16>(e[6], e[7])};
-  p1 = u32x4{pack2<F16>(e[8], e[9]), pack2<F16>(e[10], e[11]), pack2<F16>(e[12], e[13]), pack2<F16>(e[14], e[15])};
+  for (int r = 0; r < 8; ++r) e[r] = __builtin_amdgcn_exp2f(fmaf(s[8 * HALF + r], c, -shift));
+  return u32x4{pack2<F16>(e[0], e[1]), pack2<F16>(e[2], e[3]), pack2<F16>(e[4], e[5]), pack2<F16>(e[6], e[7])};
 }
 
 __device__ __forceinline__ float value16(uint16_t v, bool f16) {
@@ -350,9 +350,8 @@ __global__ __launch_bounds__(64 * kWaves) void k_paged_attn_few(Args g) {
           for (int i = 0; i < 4; ++i) va[d][u][i] = finite2<F16>(va[d][u][i], odd);
     }
     const float top = half_max(s);
-    if (above(acc, top)) raise(acc, top, c);
-    u32x4 p0, p1;
-    weights<F16>(s, c, acc.shift, p0, p1);
+    if (above(acc, top)) raise(acc, top, c, lane);
+    const u32x4 p0 = weights<F16, 0>(s, c, acc.shift), p1 = weights<F16, 1>(s, c, acc.shift);
     acc.sum = row_sum<F16>(ones, p1, row_sum<F16>(ones, p0, acc.sum));
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
@@ -399,60 +398,67 @@ __global__ __launch_bounds__(64 * kWaves) void k_paged_attn_few(Args g) {
 }
 
 // ============================================================ many columns
-// A workgroup has 4 x 32 columns, 32 a wave.  K and V stream through a ring of LDS buffers, loaded global->LDS directly
+// A workgroup has 4 x 32 QT columns, 32 QT a wave.  K and V stream through a ring of LDS buffers, loaded global->LDS directly
 // in stages of 64 (D = 64) or 32 (D = 128) keys: 16-key groups one after the other, each as the cache has it, so that
 // a wave loads one page's part of a stage.
 //
-// A unit is 32 keys.  Matrix and vector work of one unit depend on each other end to end (scores, maximum, P, P.V), so
-// a wave works on three units at once: while P of unit i is formed, the scores of i + 1 and P.V of i - 1 run on the
-// matrix pipe, in the shadow of the exponentials.  Raising the maximum, masks and infinities leave that path (rare).
-template <int D>
+// A step is 32 keys (a unit) and 32 columns.  Matrix and vector work of one step depend on each other end to end
+// (scores, maximum, P, P.V), so a wave works on three steps at once: while P of one is formed, the scores of the next
+// and P.V of the one before run on the matrix pipe, in the shadow of the exponentials.  With QT = 2 the steps of a unit
+// take turns on the two column tiles, and each K and V operand read from LDS feeds two products.  Raising the maximum,
+// masks and infinities leave that path (rare).
+template <int D, int QT>
 struct Many {
   static constexpr int kStageKeys = D == 64 ? 64 : 32, kUnits = kStageKeys / 32;  // keys and units of a stage
-  static constexpr int kAhead = D == 64 ? 1 : 2;    // stages whose loads are in flight past the one waited for
-  static constexpr int kBufs = D == 64 ? 3 : 5;     // stages: V of unit i, K of i + 2, and the ones in flight
+  static constexpr int kAhead = D == 64 && QT == 1 ? 1 : 2;  // stages whose loads are in flight past the one waited for
+  // stages in LDS: V of unit i, K of i + 2, and the ones in flight (48 KB, 64 KB or 80 KB, for 3 or 2 workgroups a CU)
+  static constexpr int kBufs = kAhead + 1 + 2 / kUnits;
   static constexpr int kGroup = 2 * D;              // 16-byte chunks of a 16-key group, K or V
   static constexpr int kStageGroups = kStageKeys / 16;
   static constexpr int kStage = 2 * kStageGroups * kGroup;  // chunks of a stage: K groups, then V groups
   static constexpr int kLoads = kStage / 64 / kWaves;       // 1 KB loads of a wave
 };
 
-template <int D, bool F16>
-__global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void k_paged_attn_many(Args g) {
-  using M = Many<D>;
+template <int D, bool F16, int QT>
+__global__ __launch_bounds__(64 * kWaves, D == 64 && QT == 1 ? 3 : 2) void k_paged_attn_many(Args g) {
+  using M = Many<D, QT>;
   constexpr int KS = D / 16, DT = D / 32;
   __shared__ u32x4 lds[M::kBufs][M::kStage];
   const int lane = threadIdx.x & 63, wave = wave_id(), j = lane & 31, hh = lane >> 5;
   Tile t;
-  if (!find_tile(g, blockIdx.x / g.kv_heads, blockIdx.x % g.kv_heads, kWaves * kCols, t)) return;
+  if (!find_tile(g, blockIdx.x / g.kv_heads, blockIdx.x % g.kv_heads, kWaves * kCols * QT, t)) return;
   const int32_t* table = g.a.table + int64_t(t.r) * g.a.max_pages;
   const float c = g.a.scale_log2;
   int s0, s1;  // stages
   split_range(g, t, M::kStageKeys, s0, s1);
   const int n_stages = max(s1 - s0, 0), n_units = n_stages * M::kUnits, first_key = s0 * M::kStageKeys;
 
-  // This wave's share of stage st: part of one group's K or V.
-  constexpr int kParts = M::kLoads * 64 < M::kGroup ? M::kGroup / (M::kLoads * 64) : 1;
-  static_assert(kParts == 1, "a wave loads whole groups");
-  constexpr int kGroupsEach = M::kLoads * 64 / M::kGroup;  // 2: K and V of one 16-key group (D = 64); 1 (D = 128)
-  const int my_group = wave % M::kStageGroups;
+  // This wave's share of stage st: K and V of one 16-key group (D = 64), or one of the two (D = 128).
+  constexpr int kGroupsEach = M::kLoads * 64 / M::kGroup;
+  static_assert(kGroupsEach * kWaves == 2 * M::kStageGroups, "a wave loads whole groups");
+  const int my_group = wave % M::kStageGroups, first_group = M::kStageGroups * s0 + my_group;
+  const uint32_t page_bytes = uint32_t(g.kv_heads) * D * 2 << g.page_shift;
+  const int64_t head = int64_t(t.h) * D << g.page_shift;
+  const uint16_t *Kh = g.a.K + head, *Vh = g.a.V + head;
   auto page_of = [&](int st) {
-    return scalar_load(table + min((M::kStageGroups * (s0 + st) + my_group) >> g.gpp_shift, g.a.max_pages - 1));
+    return scalar_load(table + min((first_group + M::kStageGroups * st) >> g.gpp_shift, g.a.max_pages - 1));
   };
+  int slot = 0;  // where the next stage goes
   auto stage = [&](int st, int page) {  // zeros for what is no page
     const bool ok = uint32_t(page) < uint32_t(g.n_pages);
-    const int in = (M::kStageGroups * (s0 + st) + my_group) & ((1 << g.gpp_shift) - 1);
-    const int64_t at = ((((int64_t(ok ? page : 0) * g.kv_heads + t.h) << g.gpp_shift) + in) * 16) * D;
+    const int in = (first_group + M::kStageGroups * st) & ((1 << g.gpp_shift) - 1);
+    const uint64_t at = uint64_t(uint32_t(ok ? page : 0)) * page_bytes + uint32_t(in * 32 * D);
     const int bytes = ok ? 32 * D : 0;
-    u32x4* dst = &lds[st % M::kBufs][my_group * M::kGroup];
+    u32x4* dst = lds[0] + slot + my_group * M::kGroup;
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
       if (kGroupsEach == 1 && v != wave / M::kStageGroups) continue;
-      const __amdgpu_buffer_rsrc_t r = buffer_rsrc((v ? g.a.V : g.a.K) + at, bytes);
+      const __amdgpu_buffer_rsrc_t r = buffer_rsrc(reinterpret_cast<const char*>(v ? Vh : Kh) + at, bytes);
 #pragma unroll
       for (int i = 0; i < M::kGroup / 64; ++i)
         buffer_load_lds16(r, (64 * i + lane) * 16, dst + v * M::kStageGroups * M::kGroup + 64 * i);
     }
+    slot = slot == (M::kBufs - 1) * M::kStage ? 0 : slot + M::kStage;
   };
   constexpr int kFirst = 2 / M::kUnits;  // stage that the end of step 0 waits for
   for (int st = 0; st < min(kFirst + M::kAhead, n_stages); ++st) stage(st, page_of(st));
@@ -465,16 +471,20 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void k_paged_attn_man
   const bool any_bad = __any(bad);
 
   // this wave's columns, and its units a .. b - 1 (counted from the workgroup's first)
-  const int col0 = t.col0 + wave * kCols, col = col0 + j;
+  const int col0 = t.col0 + wave * kCols * QT;
   const bool active = col0 < t.cols;
   int lo = 0, hi = 0, lo_all = 0, hi_all = 0;
-  if (active) key_range(g, t, col0, min(col0 + kCols, t.cols) - 1, lo, hi, lo_all, hi_all);
+  if (active) key_range(g, t, col0, min(col0 + kCols * QT, t.cols) - 1, lo, hi, lo_all, hi_all);
   const int a = min(max(lo - first_key, 0) / 32, n_units), b = min((max(hi - first_key, 0) + 31) / 32, n_units);
-  u32x4 qb[KS];
-  load_q<D>(g, t, col, hh, qb);
-  const Mask mask = mask_of(g, t, col);
-  Acc<D> acc;
-  clear(acc);
+  u32x4 qb[QT][KS];
+  Mask mask[QT];
+  Acc<D> acc[QT];
+#pragma unroll
+  for (int x = 0; x < QT; ++x) {
+    load_q<D>(g, t, col0 + kCols * x + j, hh, qb[x]);
+    mask[x] = mask_of(g, t, col0 + kCols * x + j);
+    clear(acc[x]);
+  }
   const u32x4 ones = sum_rows<F16>(lane);
 
   // places of units in the ring
@@ -503,33 +513,33 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void k_paged_attn_man
     return !any_bad || uint32_t(scalar_load(table + min(key >> 4 >> g.gpp_shift, g.a.max_pages - 1))) < uint32_t(g.n_pages);
   };
 
-  // K of unit i + 1, V and P of unit i - 1 (zeros before the first), scores of unit i
-  u32x4 ka[KS], va[DT][2], p0 = zero4(), p1 = zero4();
+  // Operands of the step after the present one (K) and of the one before it (V, P: zeros before the first), and the
+  // scores of the present step and the next.
+  u32x4 ka[KS], va[DT][2], p0[QT], p1[QT];
+  auto no_p_v = [&]() {
 #pragma unroll
-  for (int d = 0; d < DT; ++d) va[d][0] = va[d][1] = zero4();
+    for (int x = 0; x < QT; ++x) p0[x] = p1[x] = zero4();
+#pragma unroll
+    for (int d = 0; d < DT; ++d) va[d][0] = va[d][1] = zero4();
+  };
+  no_p_v();
   f32x16 s_even = zero16(), s_odd = zero16();
   auto load_k = [&](int at) {
     const u32x4* K = lds[0] + at + k_lane;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) ka[ks] = K[ks * 32];
   };
-  auto scores = [&](f32x16& s) {
+  auto scores = [&](f32x16& s, int x) {
     s = zero16();
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) s = mfma<F16>(ka[ks], qb[ks], s);
+    for (int ks = 0; ks < KS; ++ks) s = mfma<F16>(ka[ks], qb[x][ks], s);
   };
-  auto p_v = [&]() {
+  auto p_v = [&](int x) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      acc.o[d] = mfma<F16>(va[d][0], p0, acc.o[d]);
-      acc.o[d] = mfma<F16>(va[d][1], p1, acc.o[d]);
+      acc[x].o[d] = mfma<F16>(va[d][0], p0[x], acc[x].o[d]);
+      acc[x].o[d] = mfma<F16>(va[d][1], p1[x], acc[x].o[d]);
     }
-  };
-  auto settle = [&]() {  // P.V of the last unit now, and nothing of it later
-    p_v();
-    p0 = p1 = zero4();
-#pragma unroll
-    for (int d = 0; d < DT; ++d) va[d][0] = va[d][1] = zero4();
   };
 
   if (n_stages >= kFirst + M::kAhead)
@@ -540,80 +550,126 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 3 : 2) void k_paged_attn_man
   if (a < b) {
     int at = place(a), at1 = after(at, a + 1);
     load_k(at);
-    scores(s_even);
-    load_k(at1);
+    scores(s_even, 0);
+    if (QT == 1) load_k(at1);
     // units all of whose keys all columns see
-    const int w0 = (max(lo_all - first_key, 0) + 31) / 32, w1 = any_bad ? 0 : max(hi_all - first_key, 0) / 32;
-    auto step = [&](int i, f32x16& s, f32x16& s_next) {
-      const bool whole = i >= w0 && i < w1;
+    const int w0 = (max(lo_all - first_key, 0) + 31) / 32, w1 = any_bad ? 0 : min(max(hi_all - first_key, 0) / 32, b);
+    // Step of unit i and column tile x, whose scores are in s; before it came tile x of unit i - 1 (QT = 1) or the other
+    // tile.  EDGE: not all columns see all of the unit.
+    bool odd = false;  // EDGE: V of the unit has infinities or NaN, zeros in va
+    auto step = [&](auto edge, int i, int x, f32x16& s, f32x16& s_next) {
+      constexpr bool EDGE = decltype(edge)::value;
+      const bool last = x == QT - 1;
       const int key0 = first_key + 32 * i;
-      auto seen = [&](int k) { return mask(key0 + k) && group_ok(key0 + (k & 16)); };
-      if (!whole) {
+      if (EDGE) {
         const bool ok0 = group_ok(key0), ok1 = group_ok(key0 + 16);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int k = key_in_tile(r, hh);
-          s[r] = mask(key0 + k) && (k < 16 ? ok0 : ok1) ? s[r] : -INFINITY;
+          s[r] = mask[x](key0 + k) && (k < 16 ? ok0 : ok1) ? s[r] : -INFINITY;
         }
       }
       const float top = half_max(s);
-      if (above(acc, top)) {
-        settle();
-        raise(acc, top, c);
+      if (above(acc[x], top)) {
+        if (QT == 1) {  // P.V of the unit before belongs to the sums that are scaled here
+          p_v(x);
+          no_p_v();
+        }
+        raise(acc[x], top, c, lane);
       }
-      scores(s_next);
-      p_v();
-      weights<F16>(s, c, acc.shift, p0, p1);
-      acc.sum = row_sum<F16>(ones, p1, row_sum<F16>(ones, p0, acc.sum));
-      const u32x4* V = lds[0] + at + v_lane;
-#pragma unroll
-      for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) va[d][u] = V[u * M::kGroup + 32 * d];
-      if (!whole) {
-        bool odd = false;
+      // two stretches of matrix work with vector work of about its length, and the operands' loads behind each
+      scores(s_next, last ? 0 : x + 1);
+      const u32x4 n0 = weights<F16, 0>(s, c, acc[x].shift);
+      __builtin_amdgcn_sched_barrier(0);
+      if (QT == 2 && !last) load_k(at1);
+      p_v(QT - 1 - x);
+      p1[x] = weights<F16, 1>(s, c, acc[x].shift);
+      p0[x] = n0;
+      __builtin_amdgcn_sched_barrier(0);
+      acc[x].sum = row_sum<F16>(ones, p1[x], row_sum<F16>(ones, p0[x], acc[x].sum));
+      if (x == 0) {
+        const u32x4* V = lds[0] + at + v_lane;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
+          for (int u = 0; u < 2; ++u) va[d][u] = V[u * M::kGroup + 32 * d];
+        if (EDGE) {
+          bool any = false;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) va[d][u][x] = finite2<F16>(va[d][u][x], odd);
-        if (__any(odd)) {
-          settle();
-          const u32x4* unit = lds[0] + at + M::kStageGroups * M::kGroup;
-          add_infinities<D, F16>(acc, [&](int u) { return reinterpret_cast<const uint16_t*>(unit + u * M::kGroup); }, seen, hh);
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int y = 0; y < 4; ++y) va[d][u][y] = finite2<F16>(va[d][u][y], any);
+          odd = __any(any);
         }
       }
-      advance(i);
-      at = at1;
-      at1 = after(at1, i + 2);
-      load_k(at1);
+      if (EDGE && last && odd) {
+        const u32x4* unit = lds[0] + at + M::kStageGroups * M::kGroup;
+        auto group = [&](int u) { return reinterpret_cast<const uint16_t*>(unit + u * M::kGroup); };
+#pragma unroll
+        for (int y = 0; y < QT; ++y)
+          add_infinities<D, F16>(acc[y], group, [&](int k) { return mask[y](key0 + k) && group_ok(key0 + (k & 16)); }, hh);
+      }
+      if (last) {
+        advance(i);
+        at = at1;
+        at1 = after(at1, i + 2);
+        if (QT == 1) load_k(at1);
+      }
     };
-    for (int i = a; i < b; i += 2) {  // two steps a turn: the scores change places without being copied
-      step(i, s_even, s_odd);
-      if (i + 1 < b) step(i + 1, s_odd, s_even);
+    const auto inner = std::integral_constant<bool, false>{};
+    const auto edge = std::integral_constant<bool, true>{};
+    for (int i = a; i < b;) {
+      // the scores change places from step to step without being copied: two steps a turn
+      if constexpr (QT == 1) {
+        if (i >= w0)
+          for (; i + 1 < w1; i += 2) {
+            step(inner, i, 0, s_even, s_odd);
+            step(inner, i + 1, 0, s_odd, s_even);
+          }
+        if (i < b) {
+          step(edge, i++, 0, s_even, s_odd);
+          s_even = s_odd;
+        }
+      } else {
+        if (i >= w0)
+          for (; i < w1; ++i) {
+            step(inner, i, 0, s_even, s_odd);
+            step(inner, i, 1, s_odd, s_even);
+          }
+        if (i < b) {
+          step(edge, i, 0, s_even, s_odd);
+          step(edge, i++, 1, s_odd, s_even);
+        }
+      }
     }
-    p_v();
+    p_v(QT - 1);
   }
   for (int i = max(a, b); i < n_units; ++i) advance(i);
   if (!active) return;
-  const float l = sum_of(acc.sum, j);
-  if (col >= t.cols) return;
-  const int64_t out = out_row(g, t, col), part = int64_t(blockIdx.y) * g.a.n_rows * g.a.heads + out;
 #pragma unroll
-  for (int d = 0; d < DT; ++d)
+  for (int x = 0; x < QT; ++x) {
+    const int col = col0 + kCols * x + j;
+    const float l = sum_of(acc[x].sum, j);
+    if (col >= t.cols) continue;
+    const int64_t out = out_row(g, t, col), part = int64_t(blockIdx.y) * g.a.n_rows * g.a.heads + out;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f32x4 o{acc.o[d][4 * q], acc.o[d][4 * q + 1], acc.o[d][4 * q + 2], acc.o[d][4 * q + 3]};
-      const int quad = 8 * d + 2 * q + hh;
-      if (g.splits == 1)
-        store4<D, F16>(g, out, quad, o, l);
-      else
-        *reinterpret_cast<f32x4*>(g.part_o + part * D + 4 * quad) = o;
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x16& o = acc[x].o[d];
+        const f32x4 o4{o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]};
+        const int quad = 8 * d + 2 * q + hh;
+        if (g.splits == 1)
+          store4<D, F16>(g, out, quad, o4, l);
+        else
+          *reinterpret_cast<f32x4*>(g.part_o + part * D + 4 * quad) = o4;
+      }
+    if (g.splits > 1 && hh == 0) {
+      g.part_ml[2 * part] = acc[x].m;
+      g.part_ml[2 * part + 1] = l;
     }
-  if (g.splits > 1 && hh == 0) {
-    g.part_ml[2 * part] = acc.m;
-    g.part_ml[2 * part + 1] = l;
   }
 }
 
@@ -646,7 +702,7 @@ namespace {
 
 // How a call is run, from what the host knows of it.
 struct Plan {
-  bool many;  // the kernel for many columns
+  int qt;  // 0: the kernel for few columns; else 32-column tiles per wave of the one for many
   int width, tiles, search, splits;
 };
 
@@ -654,13 +710,13 @@ Plan plan_of(const PagedShape& s, const PagedAttnArgs& a) {
   Plan p{};
   const int group = a.heads / s.kv_heads;
   const int64_t most = int64_t(a.max_new) * group;  // columns of a request, at most
-  p.many = most > 32;
-  p.width = p.many ? kWaves * kCols : kCols;
+  p.qt = most <= 32 ? 0 : s.head_dim == 128 || most <= kWaves * kCols ? 1 : 2;
+  p.width = p.qt ? kWaves * kCols * p.qt : kCols;
   p.search = most > p.width;
   p.tiles = p.search ? int(int64_t(a.n_rows) * group / p.width) + a.n_requests : a.n_requests;
   // Parts of the keys: enough workgroups for four on each CU (two of the kernel for many columns), parts of 512 keys
   // at least.
-  const int64_t blocks = int64_t(p.tiles) * s.kv_heads, want = int64_t(device_cu_count()) * (p.many ? 2 : 4);
+  const int64_t blocks = int64_t(p.tiles) * s.kv_heads, want = int64_t(device_cu_count()) * (p.qt ? 2 : 4);
   p.splits = int(std::max<int64_t>(1, std::min<int64_t>({want / blocks, a.max_len / 512, 64})));
   return p;
 }
@@ -675,10 +731,12 @@ size_t paged_attention_workspace(const PagedShape& s, const PagedAttnArgs& a) {
 template <int D, bool F16>
 void launch(const Plan& p, const Args& g, hipStream_t st) {
   const dim3 grid(unsigned(int64_t(p.tiles) * g.kv_heads), unsigned(p.splits));
-  if (p.many)
-    k_paged_attn_many<D, F16><<<grid, 64 * kWaves, 0, st>>>(g);
-  else
+  if (p.qt == 0)
     k_paged_attn_few<D, F16><<<grid, 64 * kWaves, 0, st>>>(g);
+  else if (p.qt == 1)
+    k_paged_attn_many<D, F16, 1><<<grid, 64 * kWaves, 0, st>>>(g);
+  else if constexpr (D == 64)
+    k_paged_attn_many<D, F16, 2><<<grid, 64 * kWaves, 0, st>>>(g);
   if (p.splits > 1) k_paged_attn_join<D, F16><<<grid.x, 256, 0, st>>>(g, p.width);
 }
 
