@@ -1,6 +1,7 @@
 // Pages of the paged K/V cache on gfx950: dealing them to requests, taking them back, and the write of new K and V
 // rows into them (the layouts are in trf_hip.h).
 #include <algorithm>
+#include <type_traits>
 
 #include "trf_device.h"
 
@@ -9,12 +10,12 @@ namespace trf {
 // ============================================================ prefix sums over the requests
 // Every workgroup of a plan or a release forms the prefix sums over all requests itself: at most kPageRequests of
 // them, read from L2, against a second launch or a wait between workgroups.  Thread t holds requests
-// t * each .. t * each + each - 1.
-constexpr int kPageThreads = 1024;
-static_assert(kPageRequests <= 8 * kPageThreads, "requests per thread");
+// t * EACH .. t * EACH + EACH - 1 in registers.
 
 // Exclusive prefix sum over the workgroup's threads in thread order; `total` is the sum.  Sums saturate at
 // most (every term is at most most <= 2^31 - 1), which is as associative as plain addition of whole numbers.
+// lds [THREADS / 64] is not used by anything else.
+template <int THREADS>
 __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t most, uint32_t* lds, uint32_t& total) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   uint32_t incl = x;
@@ -25,12 +26,12 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t most, uint32
   }
   uint32_t excl = __shfl_up(incl, 1);
   if (lane == 0) excl = 0;
-  __syncthreads();  // the sums of an earlier call have been read
   if (lane == 63) lds[wave] = incl;
   __syncthreads();
   uint32_t before = 0;
   total = 0;
-  for (int w = 0; w < kPageThreads / 64; ++w) {
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
     if (w == wave) before = total;
     total = min(total + lds[w], most);
   }
@@ -57,58 +58,62 @@ __device__ __forceinline__ int clamped_length(int len, const PagePlan& p) {
 // ============================================================ plan
 // One thread per new row: its request by binary search over the row starts in LDS, its page from the request's
 // table row or, past the pages it has, from the pool; the row that opens a new page enters it in the table (a new
-// page's first position is always a new row).  Bound by latency: two prefix sums and one search, a few us.
-__global__ __launch_bounds__(kPageThreads) void k_page_plan(PagePlan p, const int32_t* __restrict__ state,
-                                                            const int32_t* __restrict__ n_new,
-                                                            const int32_t* __restrict__ pool, int32_t* table,
-                                                            int32_t* __restrict__ state_out,
-                                                            int32_t* __restrict__ starts, int32_t* __restrict__ slots,
-                                                            int32_t* __restrict__ positions) {
-  __shared__ uint32_t begin[kPageRequests];  // first row of each request
-  __shared__ int32_t dealt[kPageRequests];   // pages dealt before it, or -1: refused
-  __shared__ uint32_t sums[kPageThreads / 64];
-  __shared__ int32_t counts[2];              // pages dealt, requests refused
-  const int R = p.n_requests, each = (R + kPageThreads - 1) / kPageThreads;
-  const int r0 = threadIdx.x * each, r1 = min(r0 + each, R);
+// page's first position is always a new row).  Bound by latency: a read of the lengths, two prefix sums, a search and
+// a read of a page, one after the other.  Measured: 62 requests and rows {PLAN_LIVE} us, 4092 requests and 105,000 rows
+// {PLAN_SONGS} us, of which an empty kernel takes about 2.
+template <int THREADS, int EACH>
+__global__ __launch_bounds__(THREADS) void k_page_plan(PagePlan p, const int32_t* __restrict__ state,
+                                                       const int32_t* __restrict__ n_new,
+                                                       const int32_t* __restrict__ pool, int32_t* table,
+                                                       int32_t* __restrict__ state_out, int32_t* __restrict__ starts,
+                                                       int32_t* __restrict__ slots, int32_t* __restrict__ positions) {
+  __shared__ uint32_t begin[THREADS * EACH];  // first row of each request
+  __shared__ int2 request[THREADS * EACH];    // its length, and the pages dealt before it (-1: refused)
+  __shared__ uint32_t sums[2][THREADS / 64];
+  __shared__ int32_t counts[2];               // pages dealt, requests refused
+  const int R = p.n_requests, r0 = threadIdx.x * EACH, page = 1 << p.page_shift;
   const uint32_t beyond = uint32_t(p.n_rows) + 1;  // row sums end here
-  const int page = 1 << p.page_shift;
-  const int free = min(max(state[0], 0), p.n_pages);
   if (threadIdx.x < 2) counts[threadIdx.x] = 0;
-
-  uint32_t mine = 0;
-  for (int r = r0; r < r1; ++r) mine = min(mine + min(uint32_t(max(n_new[r], 0)), beyond), beyond);
-  uint32_t rows;
-  uint32_t row = block_scan(mine, beyond, sums, rows);
-  uint32_t want_mine = 0;
-  {
-    uint32_t b = row;
-    for (int r = r0; r < r1; ++r) {
-      const uint32_t n = min(uint32_t(max(n_new[r], 0)), beyond);
-      const int len = clamped_length(state[2 + r], p);
-      const bool fits = b + n < beyond && int64_t(len) + n <= int64_t(p.max_pages) << p.page_shift;
-      if (fits) want_mine += (len + n + page - 1) / page - (len + page - 1) / page;
-      begin[r] = b;
-      b = min(b + n, beyond);
-    }
+  uint32_t n[EACH], mine = 0;
+  int len[EACH];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int r = min(r0 + e, R - 1);
+    n[e] = r0 + e < R ? min(uint32_t(max(n_new[r], 0)), beyond) : 0;
+    len[e] = clamped_length(state[2 + r], p);
   }
-  uint32_t wanted;
-  uint32_t before = block_scan(want_mine, 0x7fffffffu, sums, wanted);
+  const int free = min(max(state[0], 0), p.n_pages);
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) mine = min(mine + n[e], beyond);
+  uint32_t rows, wanted;
+  uint32_t row = block_scan<THREADS>(mine, beyond, sums[0], rows);
+  uint32_t first[EACH], want[EACH], want_mine = 0;
+  bool fits[EACH];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    first[e] = row;
+    fits[e] = r0 + e < R && row + n[e] < beyond && int64_t(len[e]) + n[e] <= int64_t(p.max_pages) << p.page_shift;
+    want[e] = fits[e] ? ((len[e] + n[e] + page - 1) >> p.page_shift) - ((len[e] + page - 1) >> p.page_shift) : 0;
+    want_mine += want[e];
+    row = min(row + n[e], beyond);
+  }
+  uint32_t before = block_scan<THREADS>(want_mine, 0x7fffffffu, sums[1], wanted);
   int used = 0, refused = 0;
-  for (int r = r0; r < r1; ++r) {
-    const uint32_t b = begin[r];
-    const uint32_t n = min(uint32_t(max(n_new[r], 0)), beyond);
-    const int len = clamped_length(state[2 + r], p);
-    const bool fits = b + n < beyond && int64_t(len) + n <= int64_t(p.max_pages) << p.page_shift;
-    const uint32_t want = fits ? (len + n + page - 1) / page - (len + page - 1) / page : 0;
-    const bool ok = fits && (want == 0 || before + want <= uint32_t(free));
-    dealt[r] = ok ? int32_t(min(before, uint32_t(free))) : -1;
-    if (ok) used += want;
-    refused += !ok && n > 0;
-    if (blockIdx.x == 0) {
-      starts[r] = min(b, uint32_t(p.n_rows));
-      state_out[2 + r] = ok ? len + n : len;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int r = r0 + e;
+    const bool ok = fits[e] && (want[e] == 0 || before + want[e] <= uint32_t(free));
+    if (r < R) {
+      begin[r] = first[e];
+      request[r] = int2{len[e], ok ? int32_t(min(before, uint32_t(free))) : -1};
+      if (blockIdx.x == 0) {
+        starts[r] = min(first[e], uint32_t(p.n_rows));
+        state_out[2 + r] = ok ? len[e] + n[e] : len[e];
+      }
     }
-    before += want;
+    if (ok) used += want[e];
+    refused += !ok && n[e] > 0;
+    before += want[e];
   }
   if (blockIdx.x == 0) {
     if (used) atomicAdd(&counts[0], used);
@@ -120,24 +125,18 @@ __global__ __launch_bounds__(kPageThreads) void k_page_plan(PagePlan p, const in
     state_out[0] = free - counts[0];
     state_out[1] = counts[1];
   }
-  for (int64_t i = int64_t(blockIdx.x) * kPageThreads + threadIdx.x; i < p.n_rows; i += int64_t(gridDim.x) * kPageThreads) {
+  for (int64_t i = int64_t(blockIdx.x) * THREADS + threadIdx.x; i < p.n_rows; i += int64_t(gridDim.x) * THREADS) {
     int pos = -1, slot = -1;
     if (uint32_t(i) < rows) {
       const int r = last_not_above(begin, R, uint32_t(i));
-      const int d = dealt[r];
-      if (d >= 0) {
-        const int len = clamped_length(state[2 + r], p);
-        const int have = (len + page - 1) >> p.page_shift;
-        pos = len + int(uint32_t(i) - begin[r]);
+      const int2 q = request[r];
+      if (q.y >= 0) {
+        const int have = (q.x + page - 1) >> p.page_shift;
+        pos = q.x + int(uint32_t(i) - begin[r]);
         const int at = pos >> p.page_shift;
         int32_t* entry = table + int64_t(r) * p.max_pages + at;
-        int pg;
-        if (at < have) {
-          pg = *entry;
-        } else {
-          pg = pool[free - 1 - (d + at - have)];
-          if ((pos & (page - 1)) == 0) *entry = pg;
-        }
+        const int pg = *(at < have ? entry : pool + (free - 1 - (q.y + at - have)));
+        if (at >= have && (pos & (page - 1)) == 0) *entry = pg;
         if (uint32_t(pg) < uint32_t(p.n_pages)) slot = (pg << p.page_shift) + (pos & (page - 1));
       }
     }
@@ -146,46 +145,68 @@ __global__ __launch_bounds__(kPageThreads) void k_page_plan(PagePlan p, const in
   }
 }
 
+// Threads of a workgroup and requests of a thread: what holds them all (the fewer waves meet at a barrier the better).
+template <class Run>
+void by_requests(int32_t n, Run run) {
+  using std::integral_constant;
+  if (n <= 256)
+    run(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+  else if (n <= 1024)
+    run(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
+  else if (n <= 4096)
+    run(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
+  else
+    run(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
+}
+static_assert(kPageRequests <= 8 * 1024, "requests per thread");
+
 void launch_page_plan(const PagePlan& p, const int32_t* state, const int32_t* n_new, const int32_t* pool,
                       int32_t* table, int32_t* state_out, int32_t* starts, int32_t* slots, int32_t* positions,
                       hipStream_t st) {
-  const unsigned grid = unsigned(std::min<int64_t>(std::max<int64_t>((int64_t(p.n_rows) + 2 * kPageThreads - 1) / (2 * kPageThreads), 1), 256));
-  k_page_plan<<<grid, kPageThreads, 0, st>>>(p, state, n_new, pool, table, state_out, starts, slots, positions);
+  by_requests(p.n_requests, [&](auto threads, auto each) {
+    constexpr int T = decltype(threads)::value, E = decltype(each)::value;
+    const int64_t blocks = (int64_t(p.n_rows) + T - 1) / T;
+    const unsigned grid = unsigned(std::min<int64_t>(std::max<int64_t>(blocks, 1), 256));
+    k_page_plan<T, E><<<grid, T, 0, st>>>(p, state, n_new, pool, table, state_out, starts, slots, positions);
+  });
 }
 
 // ============================================================ release
-// One thread per released page: its request by binary search over the prefix sums in LDS.
-__global__ __launch_bounds__(kPageThreads) void k_page_release(PagePlan p, const int32_t* __restrict__ state,
-                                                               const uint8_t* __restrict__ done,
-                                                               int32_t* __restrict__ pool,
-                                                               const int32_t* __restrict__ table,
-                                                               int32_t* __restrict__ state_out) {
-  __shared__ uint32_t before[kPageRequests];  // pages released before the request's
-  __shared__ uint32_t sums[kPageThreads / 64];
-  const int R = p.n_requests, each = (R + kPageThreads - 1) / kPageThreads;
-  const int r0 = threadIdx.x * each, r1 = min(r0 + each, R);
-  const int page = 1 << p.page_shift;
+// One thread per released page: its request by binary search over the prefix sums in LDS.  Measured: 62 of 124 requests
+// {REL_LIVE} us, 1350 of 4092 with 345,000 pages {REL_SONGS} us.
+template <int THREADS, int EACH>
+__global__ __launch_bounds__(THREADS) void k_page_release(PagePlan p, const int32_t* __restrict__ state,
+                                                          const uint8_t* __restrict__ done, int32_t* __restrict__ pool,
+                                                          const int32_t* __restrict__ table,
+                                                          int32_t* __restrict__ state_out) {
+  __shared__ uint32_t before[THREADS * EACH];  // pages released before the request's
+  __shared__ uint32_t sums[THREADS / 64];
+  const int R = p.n_requests, r0 = threadIdx.x * EACH, page = 1 << p.page_shift;
   const int free = min(max(state[0], 0), p.n_pages);
-  auto pages_of = [&](int r) {
-    return done[r] ? uint32_t(clamped_length(state[2 + r], p) + page - 1) >> p.page_shift : 0u;
-  };
-  uint32_t mine = 0;
-  for (int r = r0; r < r1; ++r) mine += pages_of(r);
-  uint32_t total;
-  uint32_t at = block_scan(mine, 0x7fffffffu, sums, total);
-  for (int r = r0; r < r1; ++r) {
-    before[r] = at;
-    at += pages_of(r);
-    if (blockIdx.x == 0) state_out[2 + r] = done[r] ? 0 : clamped_length(state[2 + r], p);
+  uint32_t n[EACH], mine = 0;
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const int r = min(r0 + e, R - 1), len = clamped_length(state[2 + r], p);
+    const bool gone = done[r] != 0;
+    n[e] = r0 + e < R && gone ? uint32_t(len + page - 1) >> p.page_shift : 0;
+    if (blockIdx.x == 0 && r0 + e < R) state_out[2 + r] = gone ? 0 : len;
   }
-  const uint32_t room = uint32_t(p.n_pages - free);
-  total = min(total, room);
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) mine += n[e];
+  uint32_t total;
+  uint32_t at = block_scan<THREADS>(mine, 0x7fffffffu, sums, total);
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    if (r0 + e < R) before[r0 + e] = at;
+    at += n[e];
+  }
+  total = min(total, uint32_t(p.n_pages - free));
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     state_out[0] = free + int(total);
     state_out[1] = 0;
   }
   __syncthreads();
-  for (uint32_t k = blockIdx.x * kPageThreads + threadIdx.x; k < total; k += gridDim.x * kPageThreads) {
+  for (uint32_t k = blockIdx.x * THREADS + threadIdx.x; k < total; k += gridDim.x * THREADS) {
     const int r = last_not_above(before, R, k);
     pool[free + k] = table[int64_t(r) * p.max_pages + (k - before[r])];
   }
@@ -194,8 +215,11 @@ __global__ __launch_bounds__(kPageThreads) void k_page_release(PagePlan p, const
 void launch_page_release(const PagePlan& p, const int32_t* state, const uint8_t* done, int32_t* pool,
                          const int32_t* table, int32_t* state_out, hipStream_t st) {
   const int64_t most = std::min<int64_t>(int64_t(p.n_requests) * p.max_pages, p.n_pages);
-  const unsigned grid = unsigned(std::min<int64_t>((most + 4 * kPageThreads - 1) / (4 * kPageThreads), 128));
-  k_page_release<<<std::max(grid, 1u), kPageThreads, 0, st>>>(p, state, done, pool, table, state_out);
+  by_requests(p.n_requests, [&](auto threads, auto each) {
+    constexpr int T = decltype(threads)::value, E = decltype(each)::value;
+    const unsigned grid = unsigned(std::min<int64_t>((most + 2 * T - 1) / (2 * T), 256));
+    k_page_release<T, E><<<grid, T, 0, st>>>(p, state, done, pool, table, state_out);
+  });
 }
 
 // ============================================================ append

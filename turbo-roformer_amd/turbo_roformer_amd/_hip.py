@@ -31,6 +31,7 @@ PRECISIONS = {"bf16": PREC_BF16, "ff_split": PREC_FF_SPLIT, "ff_fp16": PREC_FF_F
 MASK_SPLIT, MASK_FP16 = 0, 1
 MASK_PRECISIONS = {"split": MASK_SPLIT, "fp16": MASK_FP16}
 _F32, _BF16, _F16 = 0, 1, 2
+_ERR_WORKSPACE = 2  # TRF_ERR_WORKSPACE
 _CACHE_DTYPES = {torch.bfloat16: _BF16, torch.float16: _F16}
 
 _lock = threading.Lock()
@@ -643,17 +644,35 @@ def overlap_finish(acc: torch.Tensor, wsum: torch.Tensor, gain: float, out: torc
 # ---------------------------------------------------------------------------------------------- paged K/V cache
 
 
-def _ints(t: torch.Tensor, name: str, shape: tuple) -> int:
-    """The address of a contiguous int32 tensor of this shape on the current device."""
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous int32 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+# One step of a live stream is a few kernels of 4-5 us each, so these wrappers keep what they do on the host short: a call
+# is 7-8 us of the host, 3 of them the launch.
+
+
+def _begin(*tensors: torch.Tensor | None) -> tuple[ctypes.CDLL, int]:
+    """The library and the current device's current stream, after checking that the tensors are on that device."""
+    lib = _lib or load()
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise ValueError(f"the tensors must be on the current device, cuda:{here}, got one on {t.device}")
+    return lib, _raw_stream(here)
+
+
+def _raw_stream(device: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device)  # current_stream() makes an object first, a us and more
+
+
+def _ints(t: torch.Tensor, name: str, *shape: int) -> int:
+    """The address of a contiguous int32 tensor of this shape."""
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 {shape}, got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 
 def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, heads: int, dim: int) -> int:
     """The row stride, in elements, of rows t [n, heads, dim] whose heads are contiguous (a slice of a projection's
     rows is)."""
-    if t.dtype != dtype or t.dim() != 3 or t.shape != (n, heads, dim):
+    if t.dtype is not dtype or t.shape != (n, heads, dim):
         raise ValueError(f"{name} must be {dtype} {(n, heads, dim)}, got {t.dtype} {tuple(t.shape)}")
     row, head, one = t.stride()
     if one != 1 or (heads > 1 and head != dim):
@@ -661,24 +680,17 @@ def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, heads: int, di
     return row if n > 1 else heads * dim
 
 
-def _here(*tensors: torch.Tensor | None) -> None:
-    """All of them are on the current device, whose current stream the call is enqueued on."""
-    here = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != here:
-            raise ValueError(f"the tensors must be on the current device, cuda:{here}, got one on {t.device}")
-
-
 def _cache(K: torch.Tensor, V: torch.Tensor) -> tuple[int, int, int, int, int]:
     """(dtype code, pages, page size, K/V heads, head dim) of a paged cache."""
-    if K.dim() != 6 or K.shape[4] != 16 or K.shape[5] != 8 or K.dtype not in _CACHE_DTYPES or not K.is_contiguous():
+    code, shape = _CACHE_DTYPES.get(K.dtype), K.shape
+    if code is None or len(shape) != 6 or shape[4:] != (16, 8) or not K.is_contiguous():
         raise ValueError("K must be contiguous bfloat16 or float16 [pages, kv heads, page size / 16, head dim / 8, 16, 8], "
-                         f"got {K.dtype} {tuple(K.shape)}")
-    pages, heads, groups, chunks = K.shape[:4]
-    if V.shape != (pages, heads, 2 * groups, 8 * chunks, 8) or V.dtype != K.dtype or not V.is_contiguous():
+                         f"got {K.dtype} {tuple(shape)}")
+    pages, heads, groups, chunks = shape[:4]
+    if V.shape != (pages, heads, 2 * groups, 8 * chunks, 8) or V.dtype is not K.dtype or not V.is_contiguous():
         raise ValueError(f"V must be contiguous {K.dtype} {(pages, heads, 2 * groups, 8 * chunks, 8)}, got {V.dtype} "
                          f"{tuple(V.shape)}")
-    return _CACHE_DTYPES[K.dtype], pages, 16 * groups, heads, 8 * chunks
+    return code, pages, 16 * groups, heads, 8 * chunks
 
 
 def paged_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
@@ -701,43 +713,41 @@ def page_plan(state, n_new, pool, table, page_size: int, state_out, starts, slot
     (free pages, refused requests, lengths) -> ``state_out``, ``table`` [R, max pages] in place, ``starts`` [R + 1],
     and for each of the rows that ``slots`` and ``positions`` have room for its slot and position, -1 where there
     is none.  All int32 on the device."""
-    lib = load()
+    lib, stream = _begin(state, n_new, pool, table, state_out, starts, slots, positions)
     R, max_pages = table.shape
-    n = slots.shape[0]
-    _here(state, n_new, pool, table, state_out, starts, slots, positions)
-    _check(lib.trf_page_plan(_ints(state, "state", (2 + R,)), _ints(n_new, "n_new", (R,)), R, n,
-                             _ints(pool, "pool", pool.shape[:1]), pool.shape[0], page_size,
-                             _ints(table, "table", (R, max_pages)), max_pages, _ints(state_out, "state_out", (2 + R,)),
-                             _ints(starts, "starts", (R + 1,)), _ints(slots, "slots", (n,)),
-                             _ints(positions, "positions", (n,)), _stream()))
+    n, pages = slots.shape[0], pool.shape[0]
+    rc = lib.trf_page_plan(_ints(state, "state", 2 + R), _ints(n_new, "n_new", R), R, n, _ints(pool, "pool", pages), pages,
+                           page_size, _ints(table, "table", R, max_pages), max_pages, _ints(state_out, "state_out", 2 + R),
+                           _ints(starts, "starts", R + 1), _ints(slots, "slots", n), _ints(positions, "positions", n), stream)
+    if rc:
+        _check(rc)
 
 
 def page_release(state, done, pool, table, page_size: int, state_out) -> None:
     """Give the pages of the requests with ``done`` [R] (bool or uint8) back to ``pool``, in place
     (``trf_page_release``): ``state`` [2 + R] -> ``state_out``, their lengths 0."""
-    lib = load()
+    lib, stream = _begin(state, done, pool, table, state_out)
     R, max_pages = table.shape
-    _here(state, done, pool, table, state_out)
+    pages = pool.shape[0]
     if done.dtype not in (torch.bool, torch.uint8) or done.shape != (R,) or not done.is_contiguous():
         raise ValueError(f"done must be contiguous bool or uint8 ({R},), got {done.dtype} {tuple(done.shape)}")
-    _check(lib.trf_page_release(_ints(state, "state", (2 + R,)), done.data_ptr(), R, _ints(pool, "pool", pool.shape[:1]),
-                                pool.shape[0], page_size, _ints(table, "table", (R, max_pages)), max_pages,
-                                _ints(state_out, "state_out", (2 + R,)), _stream()))
+    rc = lib.trf_page_release(_ints(state, "state", 2 + R), done.data_ptr(), R, _ints(pool, "pool", pages), pages, page_size,
+                              _ints(table, "table", R, max_pages), max_pages, _ints(state_out, "state_out", 2 + R), stream)
+    if rc:
+        _check(rc)
 
 
 def paged_append(k, v, K, V, slots, positions=None, rope=None, q=None, q_out=None) -> None:
     """Write rows ``k``, ``v`` [n, kv heads, head dim] (any row stride) to their ``slots`` [n] of the cache ``K``, ``V``, k
     rotated at ``positions`` [n] by the fp32 table ``rope`` [2, P, head dim / 2] (None: as it is), and ``q`` [n, heads, head
     dim] rotated likewise into ``q_out`` (``trf_paged_append``).  Rows without a slot (-1) are left out."""
-    lib = load()
+    lib, stream = _begin(k, v, K, V, slots, positions, rope, q, q_out)
     code, pages, page_size, kv, dim = _cache(K, V)
-    n = k.shape[0]
-    _here(k, v, K, V, slots, positions, rope, q, q_out)
-    ks, vs = _rows(k, "k", K.dtype, n, kv, dim), _rows(v, "v", K.dtype, n, kv, dim)
+    dtype, n = K.dtype, k.shape[0]
     heads = qs = P = 0
     if rope is not None:
         P = rope.shape[1] if rope.dim() == 3 else 0
-        if rope.dtype != torch.float32 or rope.shape != (2, P, dim // 2) or not rope.is_contiguous():
+        if rope.dtype is not torch.float32 or rope.shape != (2, P, dim // 2) or not rope.is_contiguous():
             raise ValueError(f"rope must be contiguous float32 (2, P, {dim // 2}), got {rope.dtype} {tuple(rope.shape)}")
         if positions is None:
             raise ValueError("a rotation needs positions")
@@ -745,11 +755,15 @@ def paged_append(k, v, K, V, slots, positions=None, rope=None, q=None, q_out=Non
         if q.dim() != 3 or q_out is None:
             raise ValueError("q must be [n, heads, head dim], with a q_out")
         heads = q.shape[1]
-        qs = _rows(q, "q", K.dtype, n, heads, dim)
-        _need(q_out, "q_out", K.dtype, (n, heads, dim))
-    _check(lib.trf_paged_append(_ptr(q), qs, heads, k.data_ptr(), ks, v.data_ptr(), vs, code, n, _ints(slots, "slots", (n,)),
-                                None if positions is None else _ints(positions, "positions", (n,)), _ptr(rope), P,
-                                K.data_ptr(), V.data_ptr(), pages, page_size, kv, dim, _ptr(q_out), _stream()))
+        qs = _rows(q, "q", dtype, n, heads, dim)
+        if q_out.dtype is not dtype or q_out.shape != q.shape or not q_out.is_contiguous():
+            raise ValueError(f"q_out must be contiguous {dtype} {tuple(q.shape)}, got {q_out.dtype} {tuple(q_out.shape)}")
+    rc = lib.trf_paged_append(_ptr(q), qs, heads, k.data_ptr(), _rows(k, "k", dtype, n, kv, dim), v.data_ptr(),
+                              _rows(v, "v", dtype, n, kv, dim), code, n, _ints(slots, "slots", n),
+                              None if positions is None else _ints(positions, "positions", n), _ptr(rope), P, K.data_ptr(),
+                              V.data_ptr(), pages, page_size, kv, dim, _ptr(q_out), stream)
+    if rc:
+        _check(rc)
 
 
 def paged_attention(q, K, V, table, starts, lens, O, scale: float | None = None, causal: bool = True, window: int = 0,
@@ -762,33 +776,40 @@ def paged_attention(q, K, V, table, starts, lens, O, scale: float | None = None,
     its own; ``gate`` [n, heads] fp32.  ``max_new``, ``max_len``: bounds on the rows and the length of a request (None:
     n, and what a table row holds): the tighter, the better the launch fits.  ``ws``: uint8 workspace of
     ``paged_attention_workspace_bytes`` (None: one from torch's allocator for this call)."""
-    lib = load()
+    lib, stream = _begin(q, K, V, table, starts, lens, O, gate, ws)
     code, pages, page_size, kv, dim = _cache(K, V)
+    dtype = K.dtype
     R, max_pages = table.shape
     if q.dim() != 3:
         raise ValueError(f"q must be [n, heads, head dim], got {tuple(q.shape)}")
     n, heads = q.shape[:2]
-    _here(q, K, V, table, starts, lens, O, gate, ws)
-    qs = _rows(q, "q", K.dtype, n, heads, dim)
-    if O.dtype != K.dtype or O.shape != (n, heads * dim) or not O.is_contiguous():
-        raise ValueError(f"O must be contiguous {K.dtype} {(n, heads * dim)}, got {O.dtype} {tuple(O.shape)}")
-    if gate is not None:
-        _need(gate, "gate", torch.float32, (n, heads))
+    qs = _rows(q, "q", dtype, n, heads, dim)
+    if O.dtype is not dtype or O.shape != (n, heads * dim) or not O.is_contiguous():
+        raise ValueError(f"O must be contiguous {dtype} {(n, heads * dim)}, got {O.dtype} {tuple(O.shape)}")
+    if gate is not None and (gate.dtype is not torch.float32 or gate.shape != (n, heads) or not gate.is_contiguous()):
+        raise ValueError(f"gate must be contiguous float32 {(n, heads)}, got {gate.dtype} {tuple(gate.shape)}")
     if max_new is None:
         max_new = n
     if max_len is None:
         max_len = max_pages * page_size
-    shape = (heads, code, pages, page_size, kv, dim)
-    need = lib.trf_paged_attention_workspace_bytes(*shape, max_pages, R, n, max_new, max_len)
+    ws_bytes = 0
     if ws is not None:
         _need(ws, "ws", torch.uint8)
-    elif need:
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    _check(lib.trf_paged_attention(q.data_ptr(), qs, heads, K.data_ptr(), V.data_ptr(), *shape[1:],
-                                   _ints(table, "table", (R, max_pages)), max_pages, _ints(starts, "starts", (R + 1,)),
-                                   _ints(lens, "lens", (R,)), R, n, max_new, max_len,
-                                   dim**-0.5 if scale is None else scale, int(causal), window, _ptr(gate), O.data_ptr(),
-                                   _ptr(ws), 0 if ws is None else ws.numel(), _stream()))
+        ws_bytes = ws.numel()
+    tables = (_ints(table, "table", R, max_pages), max_pages, _ints(starts, "starts", R + 1), _ints(lens, "lens", R))
+    scale = dim**-0.5 if scale is None else scale
+    while True:
+        rc = lib.trf_paged_attention(q.data_ptr(), qs, heads, K.data_ptr(), V.data_ptr(), code, pages, page_size, kv, dim,
+                                     *tables, R, n, max_new, max_len, scale, causal, window, _ptr(gate), O.data_ptr(), _ptr(ws),
+                                     ws_bytes, stream)
+        if rc == 0:
+            return
+        if rc != _ERR_WORKSPACE or ws is not None:
+            _check(rc)
+        # it is the larger calls that need one: small ones are spared the question
+        ws_bytes = lib.trf_paged_attention_workspace_bytes(heads, code, pages, page_size, kv, dim, max_pages, R, n, max_new,
+                                                           max_len)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
 
 
 def paged_attention_workspace_bytes(heads: int, K: torch.Tensor, V: torch.Tensor, n_requests: int, max_pages: int,
