@@ -223,11 +223,18 @@ void launch_page_release(const PagePlan& p, const int32_t* state, const uint8_t*
 }
 
 // ============================================================ append
-// Rows of k, v (and q) into the cache.  K keeps a position's 16-byte feature chunks 256 bytes apart and the
-// chunks of 16 positions side by side: a wave takes 16 rows and 4 chunks, holds their angles and goes through
-// the heads.  V keeps the 8 positions of an octet side by side per feature: a wave takes the rows of one octet,
-// turns them in LDS and stores 16 bytes a feature, or single values where the call does not fill the octet.
-// Bound by HBM for many rows.
+// Rows of k, v (and q) into the cache.  Memory wants a row's heads side by side where they come from, and 16 positions'
+// chunks (K) or 8 positions' values (V) side by side where they go: a workgroup reads whole rows of up to 128 features,
+// turns K on the way and lets both change direction in LDS.  It writes the 16-key groups whose first row of this call is
+// one of its 16 rows, and for that reads up to 15 rows more: the lines of a group are then written by one workgroup, whole.
+// (With rows dealt by their numbers alone two workgroups on two L2 caches write parts of the lines at each tile's end, and
+// memory has to put them together: {A17OLD} us for the first figure here.)  V goes out 16 bytes a feature, or in single values where
+// the call does not fill an octet.  Bound by HBM for many rows (a large copy reaches 5.1 TB/s): 105,462 rows of 8 heads of
+// 64 {A17} us, {A17R} TB/s; 8,700 rows of 32 and 8 heads of 128 {AP} us; 62 rows {AL} us.
+constexpr int kAppendRows = 16, kAppendFeatures = 128;
+constexpr int kMostRows = 2 * kAppendRows - 1;            // rows of the groups that a tile writes
+constexpr int kKPad = kAppendFeatures / 8 + 1;            // 16-byte chunks of a K row in LDS
+
 struct AppendArgs {
   const uint16_t *q, *k, *v;
   int64_t q_stride, k_stride, v_stride;  // elements from row to row
@@ -235,13 +242,15 @@ struct AppendArgs {
   const int32_t *slot, *position;
   const float* rope;
   uint16_t *q_out, *K, *V;
-  int32_t heads_per, qk_blocks, rows_per;
+  int32_t heads_per, parts, kv_parts;  // heads of a workgroup; workgroups per tile, and those that write K and V (the others turn q)
 };
 
-// Whether row i is written: a slot of the cache and, with a table, one of its positions.
-__device__ __forceinline__ bool live_row(const AppendArgs& a, int i, int& slot) {
-  slot = a.slot[i];
-  return uint32_t(slot) < uint32_t(a.slots) && (!a.rope || uint32_t(a.position[i]) < uint32_t(a.rope_len));
+// Row i's slot if it is written (a slot of the cache and, with a table, one of its positions), or -1.
+__device__ __forceinline__ int live_slot(const AppendArgs& a, int i) {
+  if (i < 0 || i >= a.n_rows) return -1;
+  const int slot = a.slot[i];
+  const bool live = uint32_t(slot) < uint32_t(a.slots) && (!a.rope || uint32_t(a.position[i]) < uint32_t(a.rope_len));
+  return live ? slot : -1;
 }
 
 template <bool F16>
@@ -263,96 +272,91 @@ __device__ __forceinline__ u32x4 turn8(u32x4 x, const f32x4& c, const f32x4& s) 
   return y;
 }
 
+// The 8 features from chunk c of a head on, of a row at this position, turned by the table's angles.
 template <int D, bool F16>
-__device__ __forceinline__ void append_qk(const AppendArgs& a, int block, int lane, int wave) {
-  constexpr int kParts = D / 32;                 // waves of 4 chunks that share the rows
-  constexpr int kRowTiles = 4 / kParts;          // 16-row tiles per workgroup
-  const int parts_heads = (a.heads + a.kv_heads + a.heads_per - 1) / a.heads_per;
-  const int hb = block % parts_heads, tile = (block / parts_heads) * kRowTiles + wave / kParts;
-  const int i = tile * 16 + (lane & 15), c = 4 * (wave % kParts) + (lane >> 4);
-  if (i >= a.n_rows) return;
-  int slot;
-  if (!live_row(a, i, slot)) return;
-  f32x4 cs{1.f, 1.f, 1.f, 1.f}, sn{0.f, 0.f, 0.f, 0.f};
-  if (a.rope) {
-    const float* t = a.rope + int64_t(a.position[i]) * (D / 2) + 4 * c;
-    cs = *reinterpret_cast<const f32x4*>(t);
-    sn = *reinterpret_cast<const f32x4*>(t + int64_t(a.rope_len) * (D / 2));
-  }
-  const int gpp_shift = a.page_shift - 4;
-  const int page = slot >> a.page_shift, in = slot & ((1 << a.page_shift) - 1);
-  uint16_t* Kp = a.K + (((int64_t(page) * a.kv_heads << gpp_shift) + (in >> 4)) * 16 * D + c * 128 + (in & 15) * 8);
-  const int h1 = min((hb + 1) * a.heads_per, a.heads + a.kv_heads);
-  for (int h = hb * a.heads_per; h < h1; ++h) {
-    const bool is_q = h < a.heads;
-    const uint16_t* src = is_q ? a.q + i * a.q_stride + h * D : a.k + i * a.k_stride + (h - a.heads) * D;
-    uint16_t* dst = is_q ? a.q_out + (int64_t(i) * a.heads + h) * D + 8 * c
-                         : Kp + ((int64_t(h - a.heads) << gpp_shift) * 16 * D);
-    u32x4 x = *reinterpret_cast<const u32x4*>(src + 8 * c);
-    if (a.rope) x = turn8<F16>(x, cs, sn);
-    *reinterpret_cast<u32x4*>(dst) = x;
-  }
+__device__ __forceinline__ u32x4 turned(const AppendArgs& a, u32x4 x, int position, int c) {
+  if (!a.rope) return x;
+  const float* t = a.rope + int64_t(position) * (D / 2) + 4 * c;
+  return turn8<F16>(x, *reinterpret_cast<const f32x4*>(t),
+                    *reinterpret_cast<const f32x4*>(t + int64_t(a.rope_len) * (D / 2)));
 }
 
-template <int D>
-__device__ __forceinline__ void append_v(const AppendArgs& a, int block, int lane, int wave, uint16_t* lds) {
-  constexpr int kLoads = D / 64;  // 16-byte loads per lane for 8 rows of a head
-  const int first = (block * 4 + wave) * a.rows_per;
-  const int gpp2_shift = a.page_shift - 3;
-  for (int i = first; i < min(first + a.rows_per, a.n_rows); ++i) {
-    int slot, prev;
-    if (!live_row(a, i, slot)) continue;
-    // a row that continues the octet of the row before it is written with that row
-    if ((slot & 7) && i > 0 && live_row(a, i - 1, prev) && prev == slot - 1) continue;
-    const int k8 = lane & 7;
-    int at = -1;
-    const bool in_run = k8 < 8 - (slot & 7) && i + k8 < a.n_rows && live_row(a, i + k8, at) && at == slot + k8;
-    const int run = __builtin_ctzll(~(__ballot(in_run) & 0xffull));
-    const int page = slot >> a.page_shift, in = slot & ((1 << a.page_shift) - 1);
-    uint16_t* Vp = a.V + ((int64_t(page) * a.kv_heads << gpp2_shift) + (in >> 3)) * 8 * D;
-    for (int h = 0; h < a.kv_heads; ++h) {
-      const int row = lane >> 3;
-#pragma unroll
-      for (int l = 0; l < kLoads; ++l) {
-        u32x4 x = zero4();
-        if (row < run)
-          x = *reinterpret_cast<const u32x4*>(a.v + (i + row) * a.v_stride + h * D + 64 * l + 8 * (lane & 7));
-        *reinterpret_cast<u32x4*>(lds + row * D + 64 * l + 8 * (lane & 7)) = x;
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      uint16_t* dst = Vp + (int64_t(h) << gpp2_shift) * 8 * D;
-#pragma unroll
-      for (int l = 0; l < kLoads; ++l) {
-        const int d = 64 * l + lane;
-        uint16_t e[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) e[k] = lds[k * D + d];
-        if (run == 8) {
-          u32x4 y;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) y[k] = uint32_t(e[2 * k]) | uint32_t(e[2 * k + 1]) << 16;
-          *reinterpret_cast<u32x4*>(dst + d * 8) = y;
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (k < run) dst[d * 8 + (slot & 7) + k] = e[k];
-        }
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-    }
-  }
+// What a launch writes is more than its caches hold: non-temporal stores, 165 and 160 us for the 17 s chunk, 49 and 47
+// for the pieces.
+__device__ __forceinline__ void store_once(uint16_t* dst, const u32x4& x) {
+  __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(dst));
 }
 
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
-  __shared__ u32x4 lds[4][D];  // 8 rows of D values a wave
-  const int lane = threadIdx.x & 63, wave = wave_id();
-  if (int(blockIdx.x) < a.qk_blocks)
-    append_qk<D, F16>(a, blockIdx.x, lane, wave);
-  else
-    append_v<D>(a, blockIdx.x - a.qk_blocks, lane, wave, reinterpret_cast<uint16_t*>(lds[wave]));
+  __shared__ u32x4 lds_k[kMostRows * kKPad];
+  __shared__ u32x4 lds_v[kMostRows * kAppendFeatures / 8];
+  __shared__ int2 rows[kMostRows];       // the rows that are written here, from row0 on, and their slots
+  __shared__ int32_t octets[kMostRows];  // first of their rows in that list | their number << 8
+  __shared__ int2 count;                 // rows and octets
+  constexpr int kHead = D / 8;           // chunks of a head
+  // a tile's parts run at the same time: its rows are read, and its groups written, in one go
+  const int row0 = blockIdx.x / a.parts * kAppendRows, part = blockIdx.x % a.parts, lane = threadIdx.x & 63;
+  const bool is_q = part >= a.kv_parts;
+  const int h0 = (is_q ? part - a.kv_parts : part) * a.heads_per;
+  const int nh = min(a.heads_per, (is_q ? a.heads : a.kv_heads) - h0), width = nh * kHead;  // chunks of a row
+  if (is_q) {
+    for (int x = threadIdx.x; x < kAppendRows * width; x += 256) {
+      const int r = x / width, c = x - r * width;
+      if (live_slot(a, row0 + r) < 0) continue;
+      const int64_t i = row0 + r;
+      const u32x4 y = *reinterpret_cast<const u32x4*>(a.q + i * a.q_stride + h0 * D + 8 * c);
+      store_once(a.q_out + (i * a.heads + h0) * D + 8 * c, turned<D, F16>(a, y, a.rope ? a.position[i] : 0, c % kHead));
+    }
+    return;
+  }
+  if (threadIdx.x < 64) {
+    // Lane l has row row0 - 1 + l, up to the last that a group of this tile can have.
+    const int slot = lane <= kMostRows ? live_slot(a, row0 - 1 + lane) : -1, before = __shfl_up(slot, 1);
+    // a row that continues the one before it in its group, or in its octet
+    const bool cont = lane > 0 && slot >= 0 && (slot & 15) && before == slot - 1, cont8 = cont && (slot & 7);
+    const uint64_t conts = __ballot(cont), conts8 = __ballot(cont8);
+    const int leader = 63 - __builtin_clzll((~conts & ((2ull << lane) - 1)) | 1);
+    const bool mine = slot >= 0 && leader >= 1 && leader <= kAppendRows;
+    const uint64_t mines = __ballot(mine), first8 = __ballot(mine && !cont8), below = (1ull << lane) - 1;
+    const int at = __popcll(mines & below);
+    if (mine) rows[at] = int2{lane - 1, slot};
+    if (mine && !cont8) octets[__popcll(first8 & below)] = at | (1 + __builtin_ctzll(~(conts8 >> lane >> 1))) << 8;
+    if (lane == 0) count = int2{int(__popcll(mines)), int(__popcll(first8))};
+  }
+  __syncthreads();
+  const int n_rows = count.x, n_octets = count.y;
+  for (int x = threadIdx.x; x < n_rows * width; x += 256) {
+    const int r = x / width, c = x - r * width;
+    const int64_t i = row0 + rows[r].x;
+    const u32x4 y = *reinterpret_cast<const u32x4*>(a.k + i * a.k_stride + h0 * D + 8 * c);
+    lds_v[r * (kAppendFeatures / 8) + c] = *reinterpret_cast<const u32x4*>(a.v + i * a.v_stride + h0 * D + 8 * c);
+    lds_k[r * kKPad + c] = turned<D, F16>(a, y, a.rope ? a.position[i] : 0, c % kHead);
+  }
+  __syncthreads();
+  const int page_mask = (1 << a.page_shift) - 1;
+  for (int x = threadIdx.x; x < n_rows * width; x += 256) {
+    const int c = x / n_rows, r = x - c * n_rows, slot = rows[r].y, in = slot & page_mask;
+    const int64_t head = int64_t(slot >> a.page_shift) * a.kv_heads + h0 + c / kHead;
+    uint16_t* dst = a.K + (((head << a.page_shift) + (in & ~15)) * D + (c % kHead) * 128 + (in & 15) * 8);
+    store_once(dst, lds_k[r * kKPad + c]);
+  }
+  const uint16_t* V = reinterpret_cast<const uint16_t*>(lds_v);
+  for (int x = threadIdx.x; x < n_octets * nh * D; x += 256) {
+    const int o = octets[x / (nh * D)], f = x % (nh * D), r = o & 255, n = o >> 8;
+    const int slot = rows[r].y, in = slot & page_mask;
+    const int64_t head = int64_t(slot >> a.page_shift) * a.kv_heads + h0 + f / D;
+    uint16_t* dst = a.V + (((head << a.page_shift) + (in & ~7)) * D + (f % D) * 8);
+    if (n == 8) {
+      u32x4 y;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        y[k] = uint32_t(V[(r + 2 * k) * kAppendFeatures + f]) | uint32_t(V[(r + 2 * k + 1) * kAppendFeatures + f]) << 16;
+      store_once(dst, y);
+    } else {
+      for (int k = 0; k < n; ++k) dst[(in & 7) + k] = V[(r + k) * kAppendFeatures + f];
+    }
+  }
 }
 
 void launch_paged_append(const PagedShape& s, const uint16_t* q, int64_t q_stride, int heads, const uint16_t* k,
@@ -366,15 +370,16 @@ void launch_paged_append(const PagedShape& s, const uint16_t* q, int64_t q_strid
   a.slots = s.n_pages << s.page_shift, a.page_shift = s.page_shift;
   a.slot = slots, a.position = positions, a.rope = rope;
   a.q_out = q_out, a.K = K, a.V = V;
-  a.heads_per = 4;
-  a.rows_per = n_rows > 16384 ? 8 : 1;
-  const int rows = 16 * (4 / (s.head_dim / 32));
-  const int parts = (a.heads + a.kv_heads + a.heads_per - 1) / a.heads_per;
-  a.qk_blocks = (n_rows + rows - 1) / rows * parts;
-  const unsigned grid = a.qk_blocks + (n_rows + 4 * a.rows_per - 1) / (4 * a.rows_per);
+  // Heads of a workgroup: as many as its tile holds, fewer while there are fewer than two workgroups per CU.
+  const int tiles = (n_rows + kAppendRows - 1) / kAppendRows;
+  a.heads_per = kAppendFeatures / s.head_dim;
+  auto parts = [&](int n) { return (n + a.heads_per - 1) / a.heads_per; };
+  while (a.heads_per > 1 && int64_t(tiles) * (parts(a.kv_heads) + parts(a.heads)) < 2 * device_cu_count()) a.heads_per /= 2;
+  a.kv_parts = parts(a.kv_heads);
+  a.parts = a.kv_parts + parts(a.heads);
   auto kernel = s.head_dim == 64 ? (s.f16 ? k_paged_append<64, true> : k_paged_append<64, false>)
                                  : (s.f16 ? k_paged_append<128, true> : k_paged_append<128, false>);
-  kernel<<<grid, 256, 0, st>>>(a);
+  kernel<<<unsigned(int64_t(tiles) * a.parts), 256, 0, st>>>(a);
 }
 
 }  // namespace trf
