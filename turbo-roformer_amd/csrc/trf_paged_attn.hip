@@ -290,7 +290,7 @@ __device__ __forceinline__ void split_range(const Args& g, const Tile& t, int wi
 // A workgroup has one tile of 32 columns; its four waves take every fourth 32-key tile, K and V^T operands straight
 // from the cache into registers, and join their sums in LDS at the end.
 template <int D, bool F16>
-__global__ __launch_bounds__(64 * kWaves) void k_paged_attn_few(Args g) {
+__global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void k_paged_attn_few(Args g) {
   constexpr int KS = D / 16, DT = D / 32;
   constexpr int kQuad = kCols + 1;  // columns of a feature quad in LDS, padded
   __shared__ f32x4 lds_o[kWaves][D / 4 * kQuad];
@@ -307,39 +307,43 @@ __global__ __launch_bounds__(64 * kWaves) void k_paged_attn_few(Args g) {
   const u32x4 ones = sum_rows<F16>(lane);
   const float c = g.a.scale_log2;
   const int32_t* table = g.a.table + int64_t(t.r) * g.a.max_pages;
-  const int gpp_mask = (1 << g.gpp_shift) - 1;
-  int k0, k1;
-  split_range(g, t, 32, k0, k1);
-  for (int kt = k0 + wave; kt < k1; kt += kWaves) {
-    const int key0 = kt * 32;
-    const uint16_t *Kg[2], *Vg[2];
-    bool page_ok[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int group = 2 * kt + u;
-      // the second group of the last tile may lie past the table's end
-      int page = scalar_load(table + min(group >> g.gpp_shift, g.a.max_pages - 1));
-      page_ok[u] = uint32_t(page) < uint32_t(g.n_pages);
-      if (!page_ok[u]) page = 0;
-      const int64_t base = ((((int64_t(page) * g.kv_heads + t.h) << g.gpp_shift) + (group & gpp_mask)) * 16) * D;
-      Kg[u] = g.a.K + base;
-      Vg[u] = g.a.V + base;
-    }
-    const uint16_t* Kl = (j < 16 ? Kg[0] : Kg[1]) + (hh * 16 + key_slot(j & 15)) * 8;
+  const uint32_t page_bytes = uint32_t(g.kv_heads) * D * 2 << g.page_shift;
+  const int64_t head_at = int64_t(t.h) * D << g.page_shift;
+  const uint16_t *Kh = g.a.K + head_at, *Vh = g.a.V + head_at;
+  struct Operands {
     u32x4 ka[KS], va[DT][2];
+    uint64_t at0, at1;  // elements from the head's first to the two groups, and whether they are in a page
+    bool ok0, ok1;
+  };
+  auto group_at = [&](int group, bool& ok) {
+    // the second group of the last tile may lie past the table's end
+    const int page = scalar_load(table + min(group >> g.gpp_shift, g.a.max_pages - 1));
+    ok = uint32_t(page) < uint32_t(g.n_pages);
+    return (uint64_t(uint32_t(ok ? page : 0)) * page_bytes + uint32_t((group & ((1 << g.gpp_shift) - 1)) * 32 * D)) / 2;
+  };
+  auto load = [&](Operands& x, int kt) {
+    x.at0 = group_at(2 * kt, x.ok0);
+    x.at1 = group_at(2 * kt + 1, x.ok1);
+    const uint16_t* Kl = Kh + (j < 16 ? x.at0 : x.at1) + (hh * 16 + key_slot(j & 15)) * 8;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) ka[ks] = *reinterpret_cast<const u32x4*>(Kl + ks * 256);
+    for (int ks = 0; ks < KS; ++ks) x.ka[ks] = *reinterpret_cast<const u32x4*>(Kl + ks * 256);
+    const uint16_t* Vl = Vh + (hh * D + j) * 8;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int d = 0; d < DT; ++d) va[d][u] = *reinterpret_cast<const u32x4*>(Vg[u] + (hh * D + 32 * d + j) * 8);
+    for (int d = 0; d < DT; ++d) {
+      x.va[d][0] = *reinterpret_cast<const u32x4*>(Vl + x.at0 + 256 * d);
+      x.va[d][1] = *reinterpret_cast<const u32x4*>(Vl + x.at1 + 256 * d);
+    }
+  };
+  // EDGE: not all columns see all of the tile.
+  auto tile = [&](auto edge, Operands& x, int key0) {
+    constexpr bool EDGE = decltype(edge)::value;
     f32x16 s = zero16();
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) s = mfma<F16>(ka[ks], qb[ks], s);
-    const bool whole = key0 >= t.lo_all && key0 + 32 <= t.hi_all && page_ok[0] && page_ok[1];
+    for (int ks = 0; ks < KS; ++ks) s = mfma<F16>(x.ka[ks], qb[ks], s);
     bool odd = false;  // an infinity or NaN among V that some column may not see
-    auto seen = [&](int k) { return mask(key0 + k) && page_ok[k >> 4]; };
-    if (!whole) {
+    const bool ok0 = x.ok0, ok1 = x.ok1;
+    auto seen = [&](int k) { return mask(key0 + k) && (k < 16 ? ok0 : ok1); };
+    if (EDGE) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = seen(key_in_tile(r, hh)) ? s[r] : -INFINITY;
 #pragma unroll
@@ -347,7 +351,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_paged_attn_few(Args g) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) va[d][u][i] = finite2<F16>(va[d][u][i], odd);
+          for (int i = 0; i < 4; ++i) x.va[d][u][i] = finite2<F16>(x.va[d][u][i], odd);
     }
     const float top = half_max(s);
     if (above(acc, top)) raise(acc, top, c, lane);
@@ -355,10 +359,33 @@ __global__ __launch_bounds__(64 * kWaves) void k_paged_attn_few(Args g) {
     acc.sum = row_sum<F16>(ones, p1, row_sum<F16>(ones, p0, acc.sum));
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
-      acc.o[d] = mfma<F16>(va[d][0], p0, acc.o[d]);
-      acc.o[d] = mfma<F16>(va[d][1], p1, acc.o[d]);
+      acc.o[d] = mfma<F16>(x.va[d][0], p0, acc.o[d]);
+      acc.o[d] = mfma<F16>(x.va[d][1], p1, acc.o[d]);
     }
-    if (__any(odd)) add_infinities<D, F16>(acc, [&](int u) { return Vg[u]; }, seen, hh);
+    if (EDGE && __any(odd)) {
+      const uint16_t *V0 = Vh + x.at0, *V1 = Vh + x.at1;
+      add_infinities<D, F16>(acc, [&](int u) { return u ? V1 : V0; }, seen, hh);
+    }
+  };
+  auto compute = [&](Operands& x, int kt) {
+    const int key0 = kt * 32;
+    if (key0 >= t.lo_all && key0 + 32 <= t.hi_all && x.ok0 && x.ok1)
+      tile(std::integral_constant<bool, false>{}, x, key0);
+    else
+      tile(std::integral_constant<bool, true>{}, x, key0);
+  };
+  int k0, k1;
+  split_range(g, t, 32, k0, k1);
+  Operands even, odd;
+  int kt = k0 + wave;
+  // two tiles' operands in turn: one on its way from memory while the other is worked on
+  if (kt < k1) load(even, kt);
+  for (; kt < k1; kt += 2 * kWaves) {
+    if (kt + kWaves < k1) load(odd, kt + kWaves);
+    compute(even, kt);
+    if (kt + kWaves >= k1) break;
+    if (kt + 2 * kWaves < k1) load(even, kt + 2 * kWaves);
+    compute(odd, kt + kWaves);
   }
   const float l = sum_of(acc.sum, j);
 #pragma unroll
@@ -674,28 +701,39 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && QT == 1 ? 3 : 2) void k_pag
 }
 
 // ============================================================ joining the splits
-// Splits in ascending order, so that the sums do not depend on which finished first.
+// Splits in ascending order, so that the sums do not depend on which finished first.  A workgroup has 256 / (D / 4)
+// columns, four features of one a thread; reads of all splits are under way at once (one after the other they took 20 us
+// for 25 splits).
+constexpr int kMaxSplits = 64;
+
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void k_paged_attn_join(Args g, int width) {
+  constexpr int kColumns = 256 / (D / 4);
+  __shared__ float2 ml[kMaxSplits][kColumns];
   Tile t;
   if (!find_tile(g, blockIdx.x / g.kv_heads, blockIdx.x % g.kv_heads, width, t)) return;
+  const int c0 = t.col0 + blockIdx.y * kColumns, n = min(min(kColumns, t.col0 + width - c0), t.cols - c0);
+  if (n <= 0) return;
   const int64_t stride = int64_t(g.a.n_rows) * g.a.heads;
-  for (int x = threadIdx.x; x < width * (D / 4); x += 256) {
-    const int cc = x / (D / 4), quad = x % (D / 4);
-    if (t.col0 + cc >= t.cols) break;
-    const int64_t out = out_row(g, t, t.col0 + cc);
-    float m = -INFINITY, l = 0.f;
-    for (int s = 0; s < g.splits; ++s) m = fmaxf(m, g.part_ml[2 * (s * stride + out)]);
-    f32x4 o{0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < g.splits; ++s) {
-      const int64_t at = s * stride + out;
-      const float ms = g.part_ml[2 * at];
-      const float f = ms == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((ms - m) * g.a.scale_log2);
-      l += f * g.part_ml[2 * at + 1];
-      o += f * *reinterpret_cast<const f32x4*>(g.part_o + at * D + 4 * quad);
-    }
-    store4<D, F16>(g, out, quad, o, l);
+  for (int x = threadIdx.x; x < g.splits * kColumns; x += 256) {
+    const int s = x / kColumns, cc = x % kColumns;
+    if (cc < n) ml[s][cc] = reinterpret_cast<const float2*>(g.part_ml)[s * stride + out_row(g, t, c0 + cc)];
   }
+  __syncthreads();
+  const int cc = threadIdx.x / (D / 4), quad = threadIdx.x % (D / 4);
+  if (cc >= n) return;
+  const int64_t out = out_row(g, t, c0 + cc);
+  float m = -INFINITY, l = 0.f;
+  for (int s = 0; s < g.splits; ++s) m = fmaxf(m, ml[s][cc].x);
+  f32x4 o{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int s = 0; s < g.splits; ++s) {
+    const float2 p = ml[s][cc];
+    const float f = p.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((p.x - m) * g.a.scale_log2);
+    l += f * p.y;
+    o += f * *reinterpret_cast<const f32x4*>(g.part_o + (s * stride + out) * D + 4 * quad);
+  }
+  store4<D, F16>(g, out, quad, o, l);
 }
 
 namespace {
@@ -714,10 +752,9 @@ Plan plan_of(const PagedShape& s, const PagedAttnArgs& a) {
   p.width = p.qt ? kWaves * kCols * p.qt : kCols;
   p.search = most > p.width;
   p.tiles = p.search ? int(int64_t(a.n_rows) * group / p.width) + a.n_requests : a.n_requests;
-  // Parts of the keys: enough workgroups for four on each CU (two of the kernel for many columns), parts of 512 keys
-  // at least.
-  const int64_t blocks = int64_t(p.tiles) * s.kv_heads, want = int64_t(device_cu_count()) * (p.qt ? 2 : 4);
-  p.splits = int(std::max<int64_t>(1, std::min<int64_t>({want / blocks, a.max_len / 512, 64})));
+  // Parts of the keys: enough workgroups for two on each CU, parts of 512 keys at least.
+  const int64_t blocks = int64_t(p.tiles) * s.kv_heads, want = int64_t(device_cu_count()) * 2;
+  p.splits = int(std::max<int64_t>(1, std::min<int64_t>({want / blocks, a.max_len / 512, kMaxSplits})));
   return p;
 }
 
@@ -737,7 +774,9 @@ void launch(const Plan& p, const Args& g, hipStream_t st) {
     k_paged_attn_many<D, F16, 1><<<grid, 64 * kWaves, 0, st>>>(g);
   else if constexpr (D == 64)
     k_paged_attn_many<D, F16, 2><<<grid, 64 * kWaves, 0, st>>>(g);
-  if (p.splits > 1) k_paged_attn_join<D, F16><<<grid.x, 256, 0, st>>>(g, p.width);
+  constexpr int columns = 256 / (D / 4);
+  if (p.splits > 1)
+    k_paged_attn_join<D, F16><<<dim3(grid.x, (p.width + columns - 1) / columns), 256, 0, st>>>(g, p.width);
 }
 
 void launch_paged_attention(const PagedShape& s, const PagedAttnArgs& a, void* workspace, hipStream_t st) {
