@@ -614,6 +614,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && QT == 1 ? 3 : 2) void k_pag
       p0[x] = n0;
       __builtin_amdgcn_sched_barrier(0);
       acc[x].sum = row_sum<F16>(ones, p1[x], row_sum<F16>(ones, p0[x], acc[x].sum));
+      if (QT == 1) {  // K first: the next step begins with it
+        advance(i);
+        load_k(after(at1, i + 2));
+      }
       if (x == 0) {
         const u32x4* V = lds[0] + at + v_lane;
 #pragma unroll
@@ -639,10 +643,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && QT == 1 ? 3 : 2) void k_pag
           add_infinities<D, F16>(acc[y], group, [&](int k) { return mask[y](key0 + k) && group_ok(key0 + (k & 16)); }, hh);
       }
       if (last) {
-        advance(i);
+        if (QT == 2) advance(i);
         at = at1;
         at1 = after(at1, i + 2);
-        if (QT == 1) load_k(at1);
       }
     };
     const auto inner = std::integral_constant<bool, false>{};
@@ -704,7 +707,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && QT == 1 ? 3 : 2) void k_pag
 // Splits in ascending order, so that the sums do not depend on which finished first.  A workgroup has 256 / (D / 4)
 // columns, four features of one a thread; reads of all splits are under way at once (one after the other they took 20 us
 // for 25 splits).
-constexpr int kMaxSplits = 64;
+constexpr int kMaxSplits = 32;
 
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void k_paged_attn_join(Args g, int width) {
@@ -748,13 +751,16 @@ Plan plan_of(const PagedShape& s, const PagedAttnArgs& a) {
   Plan p{};
   const int group = a.heads / s.kv_heads;
   const int64_t most = int64_t(a.max_new) * group;  // columns of a request, at most
-  p.qt = most <= 32 ? 0 : s.head_dim == 128 || most <= kWaves * kCols ? 1 : 2;
+  // Two column tiles a wave for many columns: half the LDS reads, but the last tile of 256 and the keys of a causal one
+  // waste more. us for QT = 1 and 2, 62 sequences of 1701 with 8 heads of 64: 257 columns 89 and 126, 500 129 and 138, 900
+  // 212 and 223, 1701 278 and 288, not causal 436 and 413; 8 of 8000, 2048 columns 270 and 250.
+  p.qt = most <= kCols ? 0 : s.head_dim == 128 || most <= 1024 ? 1 : 2;
   p.width = p.qt ? kWaves * kCols * p.qt : kCols;
   p.search = most > p.width;
   p.tiles = p.search ? int(int64_t(a.n_rows) * group / p.width) + a.n_requests : a.n_requests;
-  // Parts of the keys: enough workgroups for two on each CU, parts of 512 keys at least.
   const int64_t blocks = int64_t(p.tiles) * s.kv_heads, want = int64_t(device_cu_count()) * 2;
-  p.splits = int(std::max<int64_t>(1, std::min<int64_t>({want / blocks, a.max_len / 512, kMaxSplits})));
+  p.splits = int(std::min<int64_t>({want / blocks, a.max_len / 256, kMaxSplits}));
+  if (p.splits < 3) p.splits = 1;
   return p;
 }
 
