@@ -392,7 +392,7 @@ int trf_page_release(const int32_t* state, const uint8_t* done, int32_t n_reques
  * (feature pairs 2i, 2i + 1; rope = [2][rope_len][head_dim / 2] fp32, cos then sin, read at positions[row]; fp32
  * arithmetic, one rounding).  q (optional, [n_rows][heads][head_dim]) is rotated likewise into q_out (rows of
  * heads * head_dim), which may be q itself if its rows are that far apart.  Row strides are in elements, multiples
- * of 8; a row's heads are contiguous.  rope = NULL: no rotation (positions are not read).  A row whose slot is not one
+ * of 8; a row's heads are contiguous; n_rows * (heads + kv_heads) is below 2^28.  rope = NULL: no rotation (positions are not read).  A row whose slot is not one
  * of the cache, or whose position is not one of the table, is left out: nothing of it is written.  Of two rows with the
  * same slot either may be the one that is kept, value by value. */
 int trf_paged_append(const uint16_t* q, int64_t q_stride, int32_t heads, const uint16_t* k, int64_t k_stride,
@@ -414,7 +414,8 @@ size_t trf_paged_attention_workspace_bytes(int32_t heads, int32_t dtype, int32_t
  * included, does not change it.  gate [n_rows][heads] fp32 is optional (NULL: 1).  Rows of O behind the last request
  * are left as they are.
  * max_new and max_len are the caller's bounds on the rows and the length of a request, from which the launch is
- * chosen: rows past max_new may be left out, max_len bounds nothing but speed.  P is rounded to the dtype for P V,
+ * chosen: rows past max_new may be left out, max_len bounds nothing but speed.  n_rows * heads is below 2^31, and
+ * (n_rows * heads / kv_heads / 32 + n_requests) * kv_heads below 2^24.  P is rounded to the dtype for P V,
  * unnormalised; scores, their maximum and the sums are fp32.  The same call gives the same bits.
  * workspace: trf_paged_attention_workspace_bytes, 16-byte aligned, of any content, in use until the call's work is
  * done: calls that may overlap need one each. */

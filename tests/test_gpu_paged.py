@@ -242,6 +242,24 @@ def test_append_rotates_q_in_place(hip):
     _rotated_close(paged.k_rows(K.cpu())[:n], k, rope, pos, "K")
 
 
+def test_append_of_rows_with_the_same_slot_keeps_one_of_them(hip):
+    n, kv, D = 40, 2, 64
+    g = torch.Generator().manual_seed(3)
+    k, v = (torch.randn(n, kv, D, generator=g).to(BF) for _ in range(2))
+    slots = torch.arange(n)
+    slots[7], slots[30] = 20, 31  # 20 and 31 twice, 7 and 30 not at all
+    K, V = _hip.paged_cache(4, 16, kv, D, BF, DEV)
+    K.zero_(), V.zero_()
+    _hip.paged_append(k.to(DEV), v.to(DEV), K, V, slots.int().to(DEV))
+    torch.cuda.synchronize()
+    for got, want in ((paged.k_rows(K.cpu()), k), (paged.v_rows(V.cpu()), v)):
+        for s, a, b in ((20, 7, 20), (31, 30, 31)):
+            assert bool(((got[s] == want[a]) | (got[s] == want[b])).all())
+        once = [i for i in range(n) if i not in (7, 20, 30, 31)]
+        assert torch.equal(got[once], want[once])
+        assert bool((got[[7, 30]] == 0).all()) and bool((got[n:] == 0).all())
+
+
 # ---------------------------------------------------------------------------------------------- attention
 
 
@@ -291,6 +309,10 @@ ATTN = [  # lens, new, heads, kv, page
     ([1], [1], 8, 8, 64), ([17], [1], 8, 8, 16), ([33, 64, 65, 128], [1, 1, 1, 1], 4, 4, 16), ([500, 3, 1701], [1, 1, 1], 8, 2, 64),
     ([40, 100], [7, 12], 4, 4, 32), ([300, 31], [33, 31], 2, 1, 16), ([90, 70, 200], [5, 0, 65], 8, 1, 128),
     ([257], [200], 3, 3, 256), ([700, 129], [129, 129], 6, 3, 32), ([2050], [3], 16, 1, 64), ([5, 1000], [5, 300], 4, 2, 64),
+    # keys split over workgroups: single rows, some rows, many; requests far shorter than the longest
+    ([3001], [1], 2, 2, 16), ([4000, 1, 0, 260], [1, 1, 0, 1], 8, 1, 64), ([2500, 31], [40, 31], 2, 1, 32), ([1500], [300], 2, 2, 128),
+    # more than 1024 columns of a request
+    ([300, 40], [290, 3], 4, 1, 16), ([1100], [259], 8, 2, 64),
 ]
 
 
@@ -303,9 +325,10 @@ def test_attention(hip, dtype, D, lens, new, heads, kv, page):
 
 
 @pytest.mark.parametrize("causal,window", [(True, 1), (True, 16), (True, 50), (True, 10_000), (False, 0), (False, 7), (False, 33)])
-@pytest.mark.parametrize("lens,new,page", [([200, 77], [1, 1], 16), ([150, 90], [40, 90], 32), ([333], [130], 64)])
+@pytest.mark.parametrize("lens,new,page", [([200, 77], [1, 1], 16), ([150, 90], [40, 90], 32), ([333], [130], 64),
+                                           ([2100, 90], [1, 1], 16), ([1300], [45], 64), ([310], [270], 32)])
 def test_attention_masks(hip, causal, window, lens, new, page):
-    for dtype, D, heads, kv in ((BF, 64, 4, 2), (HF, 128, 2, 2)):
+    for dtype, D, heads, kv in ((BF, 64, 4, 1), (HF, 128, 2, 2)):
         c = _attn_case(lens, new, heads, kv, D, page, dtype, window + 3, padding=2)
         gate = torch.rand(c["q"].shape[0], heads, generator=torch.Generator().manual_seed(1))
         _say("attention", causal, window, lens, new, page, dtype)
@@ -340,7 +363,8 @@ def test_attention_skips_table_entries_that_are_no_pages(hip):
 
 
 @pytest.mark.parametrize("dtype", (BF, HF))
-@pytest.mark.parametrize("lens,new,page", [([50, 70], [1, 1], 64), ([100, 70, 33], [20, 40, 33], 16), ([300], [200], 32)])
+@pytest.mark.parametrize("lens,new,page", [([50, 70], [1, 1], 64), ([100, 70, 33], [20, 40, 33], 16), ([300], [200], 32),
+                                           ([1400], [3], 16), ([600], [550], 64)])
 def test_unseen_infinities_and_nan_change_nothing(hip, dtype, lens, new, page):
     """K and V are NaN and infinite wherever no row may look (behind the lengths, in free pages), and V at a position that
     some rows of a tile see and others do not: only those that see it are touched, causal, windowed or both."""
@@ -411,6 +435,29 @@ def test_attention_row_strides_and_scale(hip):
     _hip.paged_attention(wide[:, 1:4], d["K"], d["V"], d["table"], d["starts"], d["lens"], O, scale=0.3)
     torch.cuda.synchronize()
     _attn_close(O.cpu().view(n, 3, 64), c, scale=0.3)
+
+
+@pytest.mark.parametrize("new", (1, 60))
+def test_attention_workspace(hip, new):
+    """A caller's workspace: of any content, exactly as large as asked for, and refused if smaller."""
+    c = _attn_case([3000], [new], 4, 2, 64, 64, BF, 43)
+    need = _hip.paged_attention_workspace_bytes(4, c["K"], c["V"], 1, c["table"].shape[1], new, new, 3000)
+    assert need > 0
+    ws = torch.full((need + 64,), 255, dtype=torch.uint8, device=DEV)  # NaN in any type
+    kw = dict(max_new=new, max_len=3000)
+    got = _run_attn(c, ws=ws[:need], **kw)
+    assert bool((ws[need:] == 255).all())
+    _attn_close(got, c)
+    assert torch.equal(got, _run_attn(c, **kw))
+    with pytest.raises(RuntimeError, match="workspace"):
+        _run_attn(c, ws=ws[:need - 16], **kw)
+
+
+def test_attention_bounds_that_are_not_tight(hip):
+    """max_len far from the lengths, both ways, and max_new above the rows: other launches, the same result."""
+    c = _attn_case([1900, 40], [5, 2], 4, 2, 64, 64, BF, 44)
+    for kw in (dict(), dict(max_len=1), dict(max_len=1900, max_new=5), dict(max_new=7, max_len=100_000), dict(max_new=1 << 30)):
+        _attn_close(_run_attn(c, **kw), c)
 
 
 def test_attention_is_the_same_bits_again_and_at_another_place_in_the_batch(hip):

@@ -68,7 +68,7 @@ def test_plan_and_release_refuse(lib, kw, word):
     (_plan, dict(starts=None), b"starts"), (_plan, dict(slots=None), b"slots"), (_plan, dict(positions=_p(2)), b"positions"),
     (_release, dict(done=None), b"done"),
     (_append, dict(dtype=0), b"dtype"), (_append, dict(dim=96), b"head_dim"), (_append, dict(kv=0), b"kv_heads"),
-    (_append, dict(heads=0), b"heads"), (_append, dict(rows=-1), b"n_rows"), (_append, dict(rows=1 << 28), b"n_rows"),
+    (_append, dict(heads=0), b"heads"), (_append, dict(rows=-1), b"n_rows"), (_append, dict(rows=1 << 24), b"n_rows"),
     (_append, dict(k=None), b"k must"), (_append, dict(ks=516), b"multiple of 8"), (_append, dict(vs=504), b"fewer than"),
     (_append, dict(ks=0), b"fewer than"), (_append, dict(qs=256), b"fewer than"), (_append, dict(v=_p(8)), b"aligned"),
     (_append, dict(slots=None), b"slots"), (_append, dict(positions=None), b"positions"), (_append, dict(P=0), b"rope_len"),
@@ -81,7 +81,7 @@ def test_plan_and_release_refuse(lib, kw, word):
     (_attend, dict(window=-1), b"window"), (_attend, dict(causal=2), b"causal"), (_attend, dict(max_new=-1), b"max_new"),
     (_attend, dict(max_len=-1), b"max_len"), (_attend, dict(rows=1 << 28), b"n_rows"), (_attend, dict(q=None), b"q must"),
     (_attend, dict(qs=500), b"multiple of 8"), (_attend, dict(O=_p(8)), b"O must"), (_attend, dict(table=None), b"table"),
-    (_attend, dict(lens=_p(2)), b"lens"), (_attend, dict(R=1 << 28, kv=8), b"too many"), (_attend, dict(gate=_p(2)), b"gate"),
+    (_attend, dict(lens=_p(2)), b"lens"), (_attend, dict(R=1 << 21), b"too many"), (_attend, dict(gate=_p(2)), b"gate"),
 ])
 def test_refusals(lib, call, kw, word):
     assert call(lib, **kw) == 1

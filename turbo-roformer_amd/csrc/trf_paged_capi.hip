@@ -133,8 +133,8 @@ int trf_paged_append(const uint16_t* q, int64_t q_stride, int32_t heads, const u
   trf::PagedShape s{};
   TRF_TRY(check_cache(dtype, n_pages, page_size, kv_heads, head_dim, s));
   if (q && (heads < 1 || heads > 65535)) return set_error(TRF_ERR_ARG, "heads must be 1..65535, got %d", heads);
-  if (n_rows < 0 || int64_t(n_rows) * (kv_heads + (q ? heads : 0)) >= int64_t(1) << 31)
-    return set_error(TRF_ERR_ARG, "n_rows must be >= 0 and n_rows * heads below 2^31, got %d", n_rows);
+  if (n_rows < 0 || int64_t(n_rows) * (kv_heads + (q ? heads : 0)) >= int64_t(1) << 28)
+    return set_error(TRF_ERR_ARG, "n_rows must be >= 0 and n_rows * (heads + kv_heads) below 2^28, got %d", n_rows);
   if (rope && rope_len < 1) return set_error(TRF_ERR_ARG, "rope_len must be >= 1, got %d", rope_len);
   if (n_rows == 0) return TRF_OK;
   TRF_TRY(check_rows("k", k, k_stride, kv_heads, head_dim));
@@ -170,8 +170,8 @@ static int attention_args(int32_t heads, int32_t dtype, int32_t n_pages, int32_t
   if (n_rows < 0 || int64_t(n_rows) * heads >= int64_t(1) << 31)
     return set_error(TRF_ERR_ARG, "n_rows must be >= 0 and n_rows * heads below 2^31, got %d", n_rows);
   if (max_new < 0 || max_len < 0) return set_error(TRF_ERR_ARG, "max_new and max_len must be >= 0, got %d and %d", max_new, max_len);
-  // what the launch could not number: a workgroup per column tile and K/V head
-  if ((int64_t(n_rows) * (heads / kv_heads) / 32 + n_requests) * kv_heads >= int64_t(1) << 31)
+  // a workgroup of 256 threads per column tile and K/V head, and 32 bits for a launch's threads
+  if ((int64_t(n_rows) * (heads / kv_heads) / 32 + n_requests) * kv_heads >= int64_t(1) << 24)
     return set_error(TRF_ERR_ARG, "too many rows, requests and heads for one call");
   a.heads = heads;
   a.max_pages = max_pages;
