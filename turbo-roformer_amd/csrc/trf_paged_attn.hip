@@ -213,7 +213,8 @@ __device__ __forceinline__ void raise(Acc<D>& acc, float half_top, float c, int 
   acc.sum[1] *= __shfl(f, (lane & 15) + 16);
 }
 
-// Half of a tile's scores -> P as a B operand.
+// Half of a tile's scores -> P as a B operand: rounded to the type of V, as the matrix instruction takes both in one type.
+// With the sum formed from the same values (row_sum) the weights that are applied still add to one.
 template <bool F16, int HALF>
 __device__ __forceinline__ u32x4 weights(const f32x16& s, float c, float shift) {
   float e[8];
@@ -288,7 +289,11 @@ __device__ __forceinline__ void split_range(const Args& g, const Tile& t, int wi
 
 // ============================================================ few columns
 // A workgroup has one tile of 32 columns; its four waves take every fourth 32-key tile, K and V^T operands straight
-// from the cache into registers, and join their sums in LDS at the end.
+// from the cache into registers (each byte of the cache is used once, so LDS would only pass it on), and join their sums
+// in LDS at the end.  Bound by HBM, or by latency for short caches: single rows of 5 sequences of 100,000 to 131,000 keys,
+// 32 and 8 heads of 128, 398 us with the join (5.9 TB/s; one tile at a time 408 + 20, as it came first 2475); one row of 62
+// sequences of 600 to 1701 keys, 8 heads of 64, 31.6 us (4.6 TB/s: two workgroups a CU of unequal lengths); one row of 17
+// keys 5.1 us.  Head dim 128 runs one wave a SIMD, with all its registers: at two, with one tile each, 443 us.
 template <int D, bool F16>
 __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void k_paged_attn_few(Args g) {
   constexpr int KS = D / 16, DT = D / 32;
@@ -434,6 +439,14 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void k_paged_attn_few
 // and P.V of the one before run on the matrix pipe, in the shadow of the exponentials.  With QT = 2 the steps of a unit
 // take turns on the two column tiles, and each K and V operand read from LDS feeds two products.  Raising the maximum,
 // masks and infinities leave that path (rare).
+//
+// Bound by the matrix pipe beside the softmax's vector work (about 50 instructions and 16 exponentials a step, for 10
+// (D = 64) or 18 MFMAs), and by the clock that the power limit leaves, 1.9-2.1 GHz.  Measured: 62 sequences of 1701 rows
+// over 1701 keys, 8 heads of 64, 412-447 us by host (820-890 TFLOP/s; a large library matrix product reaches 1190); 9
+// sequences of 300 to 600 rows over 2400 to 5800 keys, 32 and 8 heads of 128, 292-303 us (830 TFLOP/s: 1104 workgroups in
+// 2.2 rounds of 512); 8 of 700 rows over 6000 keys 526 us (985 TFLOP/s).  Steps on the way (us for the first and the
+// second): K and V through LDS 566 and 371, three steps at once 521 and 344, two column tiles a wave and a loop without
+// edges 486 and 331.
 template <int D, int QT>
 struct Many {
   static constexpr int kStageKeys = D == 64 ? 64 : 32, kUnits = kStageKeys / 32;  // keys and units of a stage

@@ -59,8 +59,8 @@ __device__ __forceinline__ int clamped_length(int len, const PagePlan& p) {
 // One thread per new row: its request by binary search over the row starts in LDS, its page from the request's
 // table row or, past the pages it has, from the pool; the row that opens a new page enters it in the table (a new
 // page's first position is always a new row).  Bound by latency: a read of the lengths, two prefix sums, a search and
-// a read of a page, one after the other.  Measured: 62 requests and rows {PLAN_LIVE} us, 4092 requests and 105,000 rows
-// {PLAN_SONGS} us, of which an empty kernel takes about 2.
+// a read of a page, one after the other.  Measured: 62 requests and rows 3.0 us, 4092 requests and 105,000 rows 10.8
+// (with the requests read again for each step 4.1 and 14.6; 512 threads of 8 requests 13.2; 4 rows a thread 14.8).
 template <int THREADS, int EACH>
 __global__ __launch_bounds__(THREADS) void k_page_plan(PagePlan p, const int32_t* __restrict__ state,
                                                        const int32_t* __restrict__ n_new,
@@ -173,7 +173,7 @@ void launch_page_plan(const PagePlan& p, const int32_t* state, const int32_t* n_
 
 // ============================================================ release
 // One thread per released page: its request by binary search over the prefix sums in LDS.  Measured: 62 of 124 requests
-// {REL_LIVE} us, 1350 of 4092 with 345,000 pages {REL_SONGS} us.
+// 3.2 us, 1350 of 4092 with 346,000 pages 7.0.
 template <int THREADS, int EACH>
 __global__ __launch_bounds__(THREADS) void k_page_release(PagePlan p, const int32_t* __restrict__ state,
                                                           const uint8_t* __restrict__ done, int32_t* __restrict__ pool,
@@ -224,13 +224,14 @@ void launch_page_release(const PagePlan& p, const int32_t* state, const uint8_t*
 
 // ============================================================ append
 // Rows of k, v (and q) into the cache.  Memory wants a row's heads side by side where they come from, and 16 positions'
-// chunks (K) or 8 positions' values (V) side by side where they go: a workgroup reads whole rows of up to 128 features,
+// chunks (K) or 8 positions' values (V) side by side where they go: a workgroup reads rows of 128 features of k and v,
 // turns K on the way and lets both change direction in LDS.  It writes the 16-key groups whose first row of this call is
-// one of its 16 rows, and for that reads up to 15 rows more: the lines of a group are then written by one workgroup, whole.
-// (With rows dealt by their numbers alone two workgroups on two L2 caches write parts of the lines at each tile's end, and
-// memory has to put them together: {A17OLD} us for the first figure here.)  V goes out 16 bytes a feature, or in single values where
-// the call does not fill an octet.  Bound by HBM for many rows (a large copy reaches 5.1 TB/s): 105,462 rows of 8 heads of
-// 64 {A17} us, {A17R} TB/s; 8,700 rows of 32 and 8 heads of 128 {AP} us; 62 rows {AL} us.
+// one of its 16 rows, and for that reads up to 15 rows more: a group's lines are written whole, by one workgroup.  V goes
+// out 16 bytes a feature, or in single values where the call does not fill an octet.  More features a workgroup leave
+// fewer of them on a CU to cover the two waits of each (slots, then rows): us at 512, 256 and 128 features 247, 184 and
+// 165 for the 17 s chunk, 92, 65 and 49 for the pieces.  Bound by HBM for many rows, where a large copy reaches 5.1 TB/s:
+// 105,462 rows of 8 heads of 64 150 us (4.3 TB/s), 8,700 rows of 32 and 8 heads of 128 45 us (4.5 TB/s); 62 rows 4.8 us,
+// latency.
 constexpr int kAppendRows = 16, kAppendFeatures = 128;
 constexpr int kMostRows = 2 * kAppendRows - 1;            // rows of the groups that a tile writes
 constexpr int kKPad = kAppendFeatures / 8 + 1;            // 16-byte chunks of a K row in LDS
@@ -281,8 +282,8 @@ __device__ __forceinline__ u32x4 turned(const AppendArgs& a, u32x4 x, int positi
                     *reinterpret_cast<const f32x4*>(t + int64_t(a.rope_len) * (D / 2)));
 }
 
-// What a launch writes is more than its caches hold: non-temporal stores, 165 and 160 us for the 17 s chunk, 49 and 47
-// for the pieces.
+// What a large launch writes is more than the caches hold: non-temporal stores (165 and 160 us for the 17 s chunk, 49 and
+// 47 for the pieces, without and with).
 __device__ __forceinline__ void store_once(uint16_t* dst, const u32x4& x) {
   __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(dst));
 }
