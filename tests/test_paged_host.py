@@ -106,6 +106,26 @@ def test_a_cache_is_refused_before_it_is_made():
             _hip._cache(*bad)
 
 
+def test_the_module_refuses_before_any_launch(lib):
+    """Arguments that are no tensors, not on the device, of the wrong number; an address that is none."""
+    native = _hip.bind_native(lib)
+    with pytest.raises(ValueError, match="address"):
+        native.bind(1, 2, 0, 4)
+    with pytest.raises(TypeError, match="4 functions"):
+        native.bind(1)
+    ints = torch.zeros(8, dtype=torch.int32)
+    table = ints.view(2, 4)
+    for args, error, word in (
+        ((0, 0, ints, ints, ints, table, 16, ints), TypeError, "expected 11 arguments, got 8"),
+        ((0, 0, 5, ints, ints, table, 16, ints, ints, ints, ints), TypeError, "state must be a tensor, got int"),
+        ((0, 0, None, ints, ints, table, 16, ints, ints, ints, ints), TypeError, "state must be a tensor, got NoneType"),
+        ((0, 0, ints, ints, ints, table, 16, ints, ints, ints, ints), ValueError, "state is on cpu"),
+        (("x", 0, ints, ints, ints, table, 16, ints, ints, ints, ints), TypeError, "int"),
+    ):
+        with pytest.raises(error, match=word):
+            native.page_plan(*args)
+
+
 def test_oracle_layouts_and_softmax():
     """The oracle's row views invert the layouts of the header, and its attention is torch's on one request."""
     K, V = _hip.paged_cache(3, 32, 2, 64, torch.float16, "cpu")

@@ -36,6 +36,7 @@ _CACHE_DTYPES = {torch.bfloat16: _BF16, torch.float16: _F16}
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
+_native = None
 
 
 class HipUnavailable(RuntimeError):
@@ -175,8 +176,23 @@ def load() -> ctypes.CDLL:
         if not ok:
             raise HipUnavailable(reason)
         torch.cuda.init()  # the library must bind to torch's HIP runtime, loaded first
-        _lib = open_library()
+        lib = open_library()
+        bind_native(lib)
+        _lib = lib
         return _lib
+
+
+def bind_native(lib: ctypes.CDLL):
+    """The module of the paged cache's entry points (trf_python.cpp), calling this library."""
+    global _native
+    try:
+        from . import _native as native
+    except ImportError as e:
+        raise HipUnavailable(f"_native.so cannot be loaded ({e}): run `make -C turbo-roformer_amd/csrc`") from None
+    names = ("trf_page_plan", "trf_page_release", "trf_paged_append", "trf_paged_attention")
+    native.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names))
+    _native = native
+    return native
 
 
 def is_loaded() -> bool:
@@ -644,40 +660,16 @@ def overlap_finish(acc: torch.Tensor, wsum: torch.Tensor, gain: float, out: torc
 # ---------------------------------------------------------------------------------------------- paged K/V cache
 
 
-# One step of a live stream is a few kernels of 4-5 us each, so these wrappers keep what they do on the host short: a call
-# is 7-8 us of the host, 3 of them the launch.
+# One step of a live stream is a few kernels of 3-5 us each: the tensors are checked and the C functions called in
+# trf_python.cpp, under 1 us of the host a call where these checks and ctypes took 5.
 
 
-def _begin(*tensors: torch.Tensor | None) -> tuple[ctypes.CDLL, int]:
-    """The library and the current device's current stream, after checking that the tensors are on that device."""
-    lib = _lib or load()
-    here = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and t.get_device() != here:
-            raise ValueError(f"the tensors must be on the current device, cuda:{here}, got one on {t.device}")
-    return lib, _raw_stream(here)
-
-
-def _raw_stream(device: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(device)  # current_stream() makes an object first, a us and more
-
-
-def _ints(t: torch.Tensor, name: str, *shape: int) -> int:
-    """The address of a contiguous int32 tensor of this shape."""
-    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous int32 {shape}, got {t.dtype} {tuple(t.shape)}")
-    return t.data_ptr()
-
-
-def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, n: int, heads: int, dim: int) -> int:
-    """The row stride, in elements, of rows t [n, heads, dim] whose heads are contiguous (a slice of a projection's
-    rows is)."""
-    if t.dtype is not dtype or t.shape != (n, heads, dim):
-        raise ValueError(f"{name} must be {dtype} {(n, heads, dim)}, got {t.dtype} {tuple(t.shape)}")
-    row, head, one = t.stride()
-    if one != 1 or (heads > 1 and head != dim):
-        raise ValueError(f"{name}'s heads must be contiguous in a row, got strides {t.stride()}")
-    return row if n > 1 else heads * dim
+def _here() -> tuple:
+    """The module of the entry points, the current device and its current stream."""
+    if _native is None:
+        load()
+    device = torch.cuda.current_device()
+    return _native, device, torch._C._cuda_getCurrentRawStream(device)  # current_stream() makes an object first, a us
 
 
 def _cache(K: torch.Tensor, V: torch.Tensor) -> tuple[int, int, int, int, int]:
@@ -713,12 +705,8 @@ def page_plan(state, n_new, pool, table, page_size: int, state_out, starts, slot
     (free pages, refused requests, lengths) -> ``state_out``, ``table`` [R, max pages] in place, ``starts`` [R + 1],
     and for each of the rows that ``slots`` and ``positions`` have room for its slot and position, -1 where there
     is none.  All int32 on the device."""
-    lib, stream = _begin(state, n_new, pool, table, state_out, starts, slots, positions)
-    R, max_pages = table.shape
-    n, pages = slots.shape[0], pool.shape[0]
-    rc = lib.trf_page_plan(_ints(state, "state", 2 + R), _ints(n_new, "n_new", R), R, n, _ints(pool, "pool", pages), pages,
-                           page_size, _ints(table, "table", R, max_pages), max_pages, _ints(state_out, "state_out", 2 + R),
-                           _ints(starts, "starts", R + 1), _ints(slots, "slots", n), _ints(positions, "positions", n), stream)
+    native, device, stream = _here()
+    rc = native.page_plan(device, stream, state, n_new, pool, table, page_size, state_out, starts, slots, positions)
     if rc:
         _check(rc)
 
@@ -726,13 +714,8 @@ def page_plan(state, n_new, pool, table, page_size: int, state_out, starts, slot
 def page_release(state, done, pool, table, page_size: int, state_out) -> None:
     """Give the pages of the requests with ``done`` [R] (bool or uint8) back to ``pool``, in place
     (``trf_page_release``): ``state`` [2 + R] -> ``state_out``, their lengths 0."""
-    lib, stream = _begin(state, done, pool, table, state_out)
-    R, max_pages = table.shape
-    pages = pool.shape[0]
-    if done.dtype not in (torch.bool, torch.uint8) or done.shape != (R,) or not done.is_contiguous():
-        raise ValueError(f"done must be contiguous bool or uint8 ({R},), got {done.dtype} {tuple(done.shape)}")
-    rc = lib.trf_page_release(_ints(state, "state", 2 + R), done.data_ptr(), R, _ints(pool, "pool", pages), pages, page_size,
-                              _ints(table, "table", R, max_pages), max_pages, _ints(state_out, "state_out", 2 + R), stream)
+    native, device, stream = _here()
+    rc = native.page_release(device, stream, state, done, pool, table, page_size, state_out)
     if rc:
         _check(rc)
 
@@ -741,27 +724,8 @@ def paged_append(k, v, K, V, slots, positions=None, rope=None, q=None, q_out=Non
     """Write rows ``k``, ``v`` [n, kv heads, head dim] (any row stride) to their ``slots`` [n] of the cache ``K``, ``V``, k
     rotated at ``positions`` [n] by the fp32 table ``rope`` [2, P, head dim / 2] (None: as it is), and ``q`` [n, heads, head
     dim] rotated likewise into ``q_out`` (``trf_paged_append``).  Rows without a slot (-1) are left out."""
-    lib, stream = _begin(k, v, K, V, slots, positions, rope, q, q_out)
-    code, pages, page_size, kv, dim = _cache(K, V)
-    dtype, n = K.dtype, k.shape[0]
-    heads = qs = P = 0
-    if rope is not None:
-        P = rope.shape[1] if rope.dim() == 3 else 0
-        if rope.dtype is not torch.float32 or rope.shape != (2, P, dim // 2) or not rope.is_contiguous():
-            raise ValueError(f"rope must be contiguous float32 (2, P, {dim // 2}), got {rope.dtype} {tuple(rope.shape)}")
-        if positions is None:
-            raise ValueError("a rotation needs positions")
-    if q is not None:
-        if q.dim() != 3 or q_out is None:
-            raise ValueError("q must be [n, heads, head dim], with a q_out")
-        heads = q.shape[1]
-        qs = _rows(q, "q", dtype, n, heads, dim)
-        if q_out.dtype is not dtype or q_out.shape != q.shape or not q_out.is_contiguous():
-            raise ValueError(f"q_out must be contiguous {dtype} {tuple(q.shape)}, got {q_out.dtype} {tuple(q_out.shape)}")
-    rc = lib.trf_paged_append(_ptr(q), qs, heads, k.data_ptr(), _rows(k, "k", dtype, n, kv, dim), v.data_ptr(),
-                              _rows(v, "v", dtype, n, kv, dim), code, n, _ints(slots, "slots", n),
-                              None if positions is None else _ints(positions, "positions", n), _ptr(rope), P, K.data_ptr(),
-                              V.data_ptr(), pages, page_size, kv, dim, _ptr(q_out), stream)
+    native, device, stream = _here()
+    rc = native.paged_append(device, stream, k, v, K, V, slots, positions, rope, q, q_out)
     if rc:
         _check(rc)
 
@@ -776,40 +740,17 @@ def paged_attention(q, K, V, table, starts, lens, O, scale: float | None = None,
     its own; ``gate`` [n, heads] fp32.  ``max_new``, ``max_len``: bounds on the rows and the length of a request (None:
     n, and what a table row holds): the tighter, the better the launch fits.  ``ws``: uint8 workspace of
     ``paged_attention_workspace_bytes`` (None: one from torch's allocator for this call)."""
-    lib, stream = _begin(q, K, V, table, starts, lens, O, gate, ws)
-    code, pages, page_size, kv, dim = _cache(K, V)
-    dtype = K.dtype
-    R, max_pages = table.shape
-    if q.dim() != 3:
-        raise ValueError(f"q must be [n, heads, head dim], got {tuple(q.shape)}")
-    n, heads = q.shape[:2]
-    qs = _rows(q, "q", dtype, n, heads, dim)
-    if O.dtype is not dtype or O.shape != (n, heads * dim) or not O.is_contiguous():
-        raise ValueError(f"O must be contiguous {dtype} {(n, heads * dim)}, got {O.dtype} {tuple(O.shape)}")
-    if gate is not None and (gate.dtype is not torch.float32 or gate.shape != (n, heads) or not gate.is_contiguous()):
-        raise ValueError(f"gate must be contiguous float32 {(n, heads)}, got {gate.dtype} {tuple(gate.shape)}")
-    if max_new is None:
-        max_new = n
-    if max_len is None:
-        max_len = max_pages * page_size
-    ws_bytes = 0
-    if ws is not None:
-        _need(ws, "ws", torch.uint8)
-        ws_bytes = ws.numel()
-    tables = (_ints(table, "table", R, max_pages), max_pages, _ints(starts, "starts", R + 1), _ints(lens, "lens", R))
-    scale = dim**-0.5 if scale is None else scale
-    while True:
-        rc = lib.trf_paged_attention(q.data_ptr(), qs, heads, K.data_ptr(), V.data_ptr(), code, pages, page_size, kv, dim,
-                                     *tables, R, n, max_new, max_len, scale, causal, window, _ptr(gate), O.data_ptr(), _ptr(ws),
-                                     ws_bytes, stream)
-        if rc == 0:
-            return
-        if rc != _ERR_WORKSPACE or ws is not None:
-            _check(rc)
-        # it is the larger calls that need one: small ones are spared the question
-        ws_bytes = lib.trf_paged_attention_workspace_bytes(heads, code, pages, page_size, kv, dim, max_pages, R, n, max_new,
-                                                           max_len)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    native, device, stream = _here()
+    rc = native.paged_attention(device, stream, q, K, V, table, starts, lens, O, scale, causal, window, gate, max_new, max_len, ws)
+    if rc == _ERR_WORKSPACE and ws is None:  # it is the larger calls that need one: small ones are spared the question
+        n, heads = q.shape[:2]
+        need = paged_attention_workspace_bytes(heads, K, V, *table.shape, n, n if max_new is None else max_new,
+                                               (1 << 31) - 1 if max_len is None else max_len)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        rc = native.paged_attention(device, stream, q, K, V, table, starts, lens, O, scale, causal, window, gate, max_new, max_len,
+                                    ws)
+    if rc:
+        _check(rc)
 
 
 def paged_attention_workspace_bytes(heads: int, K: torch.Tensor, V: torch.Tensor, n_requests: int, max_pages: int,
