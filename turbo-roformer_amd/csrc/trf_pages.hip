@@ -12,30 +12,43 @@ namespace trf {
 // them, read from L2, against a second launch or a wait between workgroups.  Thread t holds requests
 // t * EACH .. t * EACH + EACH - 1 in registers.
 
-// Exclusive prefix sum over the workgroup's threads in thread order; `total` is the sum.  Sums saturate at
-// most (every term is at most most <= 2^31 - 1), which is as associative as plain addition of whole numbers.
-// lds [THREADS / 64] is not used by anything else.
+// x of the lane that a DPP control names, 0 where there is none or the row is not in the mask.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t lane_before(uint32_t x) {
+  return uint32_t(__builtin_amdgcn_update_dpp(0, int(x), CTRL, ROWS, 0xf, false));
+}
+
+// Inclusive prefix sum over the wave: within rows of 16 lanes, then of each row's last lane into the rows behind it.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x, uint32_t most) {
+  x = min(x + lane_before<0x111, 0xf>(x), most);  // row_shr:1, 2, 4, 8
+  x = min(x + lane_before<0x112, 0xf>(x), most);
+  x = min(x + lane_before<0x114, 0xf>(x), most);
+  x = min(x + lane_before<0x118, 0xf>(x), most);
+  x = min(x + lane_before<0x142, 0xa>(x), most);  // row_bcast:15 into rows 1 and 3
+  return min(x + lane_before<0x143, 0xc>(x), most);  // row_bcast:31 into rows 2 and 3
+}
+
+// Exclusive prefix sums of x and y over the workgroup's threads in thread order, and their totals.  Sums saturate at
+// most_x and most_y (every term is at most that, and that at most 2^31 - 1), which is as associative as plain addition of
+// whole numbers.  lds [2][THREADS / 64] is not used by anything else until the next barrier.
 template <int THREADS>
-__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t most, uint32_t* lds, uint32_t& total) {
+__device__ __forceinline__ void block_scan(uint32_t& x, uint32_t& y, uint32_t most_x, uint32_t most_y, uint32_t* lds,
+                                           uint32_t& total_x, uint32_t& total_y) {
+  constexpr int W = THREADS / 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint32_t incl = x;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t y = __shfl_up(incl, d);
-    if (lane >= d) incl = min(incl + y, most);
-  }
-  uint32_t excl = __shfl_up(incl, 1);
-  if (lane == 0) excl = 0;
-  if (lane == 63) lds[wave] = incl;
+  const uint32_t in_x = wave_scan(x, most_x), in_y = wave_scan(y, most_y);
+  if (lane == 63) lds[wave] = in_x, lds[W + wave] = in_y;
   __syncthreads();
-  uint32_t before = 0;
-  total = 0;
+  uint32_t before_x = 0, before_y = 0;
+  total_x = total_y = 0;
 #pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) {
-    if (w == wave) before = total;
-    total = min(total + lds[w], most);
+  for (int w = 0; w < W; ++w) {
+    if (w == wave) before_x = total_x, before_y = total_y;
+    total_x = min(total_x + lds[w], most_x);
+    total_y = min(total_y + lds[W + w], most_y);
   }
-  return min(before + excl, most);
+  x = min(before_x + lane_before<0x138, 0xf>(in_x), most_x);  // wave_shr:1
+  y = min(before_y + lane_before<0x138, 0xf>(in_y), most_y);
 }
 
 // Last index r in [0, n) with a[r] <= v, for ascending a with a[0] <= v.
@@ -69,7 +82,7 @@ __global__ __launch_bounds__(THREADS) void k_page_plan(PagePlan p, const int32_t
                                                        int32_t* __restrict__ slots, int32_t* __restrict__ positions) {
   __shared__ uint32_t begin[THREADS * EACH];  // first row of each request
   __shared__ int2 request[THREADS * EACH];    // its length, and the pages dealt before it (-1: refused)
-  __shared__ uint32_t sums[2][THREADS / 64];
+  __shared__ uint32_t sums[2][2 * THREADS / 64];
   __shared__ int32_t counts[2];               // pages dealt, requests refused
   const int R = p.n_requests, r0 = threadIdx.x * EACH, page = 1 << p.page_shift;
   const uint32_t beyond = uint32_t(p.n_rows) + 1;  // row sums end here
@@ -83,21 +96,37 @@ __global__ __launch_bounds__(THREADS) void k_page_plan(PagePlan p, const int32_t
     len[e] = clamped_length(state[2 + r], p);
   }
   const int free = min(max(state[0], 0), p.n_pages);
-#pragma unroll
-  for (int e = 0; e < EACH; ++e) mine = min(mine + n[e], beyond);
-  uint32_t rows, wanted;
-  uint32_t row = block_scan<THREADS>(mine, beyond, sums[0], rows);
-  uint32_t first[EACH], want[EACH], want_mine = 0;
+  // Pages are wanted by requests whose rows fit; that they all do is what both sums are formed on at once.
+  const int64_t cap = int64_t(p.max_pages) << p.page_shift;
+  uint32_t want[EACH], want_mine = 0;
   bool fits[EACH];
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
-    first[e] = row;
-    fits[e] = r0 + e < R && row + n[e] < beyond && int64_t(len[e]) + n[e] <= int64_t(p.max_pages) << p.page_shift;
+    fits[e] = r0 + e < R && int64_t(len[e]) + n[e] <= cap;
     want[e] = fits[e] ? ((len[e] + n[e] + page - 1) >> p.page_shift) - ((len[e] + page - 1) >> p.page_shift) : 0;
     want_mine += want[e];
+    mine = min(mine + n[e], beyond);
+  }
+  uint32_t row = mine, before = want_mine, rows, wanted;
+  block_scan<THREADS>(row, before, beyond, 0x7fffffffu, sums[0], rows, wanted);
+  uint32_t first[EACH];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    first[e] = row;
     row = min(row + n[e], beyond);
   }
-  uint32_t before = block_scan<THREADS>(want_mine, 0x7fffffffu, sums[1], wanted);
+  if (rows == beyond) {  // more rows than there is room for: once more, without the requests that do not fit
+    want_mine = 0;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      fits[e] &= first[e] + n[e] < beyond;
+      if (!fits[e]) want[e] = 0;
+      want_mine += want[e];
+    }
+    uint32_t none = 0;
+    before = want_mine;
+    block_scan<THREADS>(before, none, 0x7fffffffu, 0, sums[1], wanted, none);
+  }
   int used = 0, refused = 0;
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
@@ -180,7 +209,7 @@ __global__ __launch_bounds__(THREADS) void k_page_release(PagePlan p, const int3
                                                           const int32_t* __restrict__ table,
                                                           int32_t* __restrict__ state_out) {
   __shared__ uint32_t before[THREADS * EACH];  // pages released before the request's
-  __shared__ uint32_t sums[THREADS / 64];
+  __shared__ uint32_t sums[2 * THREADS / 64];
   const int R = p.n_requests, r0 = threadIdx.x * EACH, page = 1 << p.page_shift;
   const int free = min(max(state[0], 0), p.n_pages);
   uint32_t n[EACH], mine = 0;
@@ -193,8 +222,8 @@ __global__ __launch_bounds__(THREADS) void k_page_release(PagePlan p, const int3
   }
 #pragma unroll
   for (int e = 0; e < EACH; ++e) mine += n[e];
-  uint32_t total;
-  uint32_t at = block_scan<THREADS>(mine, 0x7fffffffu, sums, total);
+  uint32_t at = mine, none = 0, total;
+  block_scan<THREADS>(at, none, 0x7fffffffu, 0, sums, total, none);
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
     if (r0 + e < R) before[r0 + e] = at;
