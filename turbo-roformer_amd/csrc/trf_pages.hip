@@ -325,8 +325,10 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
   __shared__ int32_t octets[kMostRows];  // first of their rows in that list | their number << 8
   __shared__ int2 count;                 // rows and octets
   constexpr int kHead = D / 8;           // chunks of a head
-  // a tile's parts run at the same time: its rows are read, and its groups written, in one go
-  const int row0 = blockIdx.x / a.parts * kAppendRows, part = blockIdx.x % a.parts, lane = threadIdx.x & 63;
+  // A tile's parts run at the same time: its rows are read, and its groups written, in one go.  Workgroups are dealt to
+  // the 8 XCDs in turn, and parts that write K and V move twice what the others do: the parts start one later in each tile.
+  const int tile = blockIdx.x / a.parts, row0 = tile * kAppendRows, lane = threadIdx.x & 63;
+  const int part = int((blockIdx.x + tile) % uint32_t(a.parts));
   const bool is_q = part >= a.kv_parts;
   const int h0 = (is_q ? part - a.kv_parts : part) * a.heads_per;
   const int nh = min(a.heads_per, (is_q ? a.heads : a.kv_heads) - h0), width = nh * kHead;  // chunks of a row
