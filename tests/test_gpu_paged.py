@@ -311,6 +311,9 @@ ATTN = [  # lens, new, heads, kv, page
     ([257], [200], 3, 3, 256), ([700, 129], [129, 129], 6, 3, 32), ([2050], [3], 16, 1, 64), ([5, 1000], [5, 300], 4, 2, 64),
     # keys split over workgroups: single rows, some rows, many; requests far shorter than the longest
     ([3001], [1], 2, 2, 16), ([4000, 1, 0, 260], [1, 1, 0, 1], 8, 1, 64), ([2500, 31], [40, 31], 2, 1, 32), ([1500], [300], 2, 2, 128),
+    # column tiles of more than 64 requests, and of requests of one length
+    ([(37 * i) % 90 + 1 for i in range(70)], [min((37 * i) % 90 + 1, (13 * i) % 43) for i in range(70)], 4, 1, 16),
+    ([200] * 5, [60, 3, 0, 45, 70], 4, 1, 32),
     # more than 1024 columns of a request
     ([300, 40], [290, 3], 4, 1, 16), ([1100], [259], 8, 2, 64),
 ]

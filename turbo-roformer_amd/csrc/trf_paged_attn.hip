@@ -27,7 +27,8 @@ constexpr float kRaise = 8.0f;
 struct Args {
   PagedAttnArgs a;
   int32_t n_pages, kv_heads, group, gpp_shift, page_shift;  // gpp_shift: log2 of the 16-key groups of a page
-  int32_t search;  // column tiles are numbered over all requests (0: a request has one)
+  int32_t search;  // column tiles are numbered over all requests: 1 in their order, 2 the ones with most keys first (0: a
+                   // request has one)
   int32_t splits;  // parts that a tile's keys are cut into, each a workgroup's
   float* part_o;   // splits > 1: O before the division, [split][row][head][D] ...
   float* part_ml;  // ... and (m, l), [split][row][head][2]
@@ -92,6 +93,30 @@ __device__ __forceinline__ int request_of_tile(const Args& g, int t, int width, 
   return lo;
 }
 
+// The same for at most 64 requests, in the order of the keys that their tiles see, most first: with a few rounds of
+// workgroups of unequal lengths the long ones must not come last (us, in their order and so: 62 sequences of 200 to 4000
+// keys, 50 to 200 rows 87 and 75; 16 of 1000 to 8000, 500 to 1000 rows 193 and 158).  A lane has a request.  False: all
+// see as many, and their order will do.  r: -1 for a tile past the last; at: the tile's number within the request.
+__device__ __forceinline__ bool request_by_length(const Args& g, int t, int width, int& r, int& at) {
+  const int lane = threadIdx.x & 63, R = g.a.n_requests, mine = min(lane, R - 1);
+  const int s0 = min(max(g.a.starts[mine], 0), g.a.n_rows), n = min(max(g.a.starts[mine + 1], s0), g.a.n_rows) - s0;
+  const int len = min(max(g.a.lens[mine], 0), g.a.max_pages << g.page_shift);
+  const int keys = g.a.window ? int(min(int64_t(len), int64_t(n) + g.a.window)) : len;
+  if (__all(keys == __builtin_amdgcn_readfirstlane(keys))) return false;
+  const int tiles = lane < R ? int((int64_t(n) * g.group + width - 1) / width) : 0;
+  // keys (of 2^25 at most) and, for equal ones, the request: no two the same
+  const int order = min(keys, (1 << 25) - 1) << 6 | (63 - lane);
+  int first = 0;
+#pragma unroll 4
+  for (int q = 0; q < R; ++q)
+    first += __builtin_amdgcn_readlane(order, q) > order ? __builtin_amdgcn_readlane(tiles, q) : 0;
+  const uint64_t found = __ballot(t >= first && t < first + tiles);
+  r = found ? __builtin_ctzll(found) : -1;
+  // a causal request's last rows see the most
+  if (found) at = __builtin_amdgcn_readlane(tiles, r) - 1 - (t - __builtin_amdgcn_readlane(first, r));
+  return true;
+}
+
 __device__ __forceinline__ int clamp_key(const Tile& t, int64_t x) { return int(min(max(x, int64_t(0)), int64_t(t.len))); }
 
 // Keys that any and all of the columns col0 .. last of the tile's request see.
@@ -108,7 +133,9 @@ __device__ __forceinline__ bool find_tile(const Args& g, int tile, int h, int wi
   int k = 0;
   t.r = tile;
   t.h = h;
-  if (g.search) {
+  if (g.search == 2 && request_by_length(g, tile, width, t.r, k)) {
+    if (t.r < 0) return false;
+  } else if (g.search) {
     int base;
     t.r = __builtin_amdgcn_readfirstlane(request_of_tile(g, tile, width, base));
     k = tile - __builtin_amdgcn_readfirstlane(base);
@@ -774,6 +801,8 @@ Plan plan_of(const PagedShape& s, const PagedAttnArgs& a) {
   const int64_t blocks = int64_t(p.tiles) * s.kv_heads, want = int64_t(device_cu_count()) * 2;
   p.splits = int(std::min<int64_t>({want / blocks, a.max_len / 256, kMaxSplits}));
   if (p.splits < 3) p.splits = 1;
+  // Requests by length where it matters: beyond some rounds of two workgroups a CU the last one is a small part of all.
+  if (p.search && a.n_requests > 1 && a.n_requests <= 64 && blocks < 6 * want) p.search = 2;
   return p;
 }
 
