@@ -72,8 +72,9 @@ __device__ __forceinline__ int clamped_length(int len, const PagePlan& p) {
 // One thread per new row: its request by binary search over the row starts in LDS, its page from the request's
 // table row or, past the pages it has, from the pool; the row that opens a new page enters it in the table (a new
 // page's first position is always a new row).  Bound by latency: a read of the lengths, two prefix sums, a search and
-// a read of a page, one after the other.  Measured: 62 requests and rows 3.0 us, 4092 requests and 105,000 rows 10.8
-// (with the requests read again for each step 4.1 and 14.6; 512 threads of 8 requests 13.2; 4 rows a thread 14.8).
+// a read of a page, one after the other.  Measured: 62 requests and rows 2.5 us, 4092 requests and 105,000 rows 9.4 (one
+// sum after the other 3.0 and 10.8, and with the requests read again for each step 4.1 and 14.6; 512 threads of 8
+// requests 13.2, 4 rows a thread 14.8).
 template <int THREADS, int EACH>
 __global__ __launch_bounds__(THREADS) void k_page_plan(PagePlan p, const int32_t* __restrict__ state,
                                                        const int32_t* __restrict__ n_new,
@@ -202,7 +203,7 @@ void launch_page_plan(const PagePlan& p, const int32_t* state, const int32_t* n_
 
 // ============================================================ release
 // One thread per released page: its request by binary search over the prefix sums in LDS.  Measured: 62 of 124 requests
-// 3.2 us, 1350 of 4092 with 346,000 pages 7.0.
+// 3.0 us, 1350 of 4092 with 346,000 pages 6.4.
 template <int THREADS, int EACH>
 __global__ __launch_bounds__(THREADS) void k_page_release(PagePlan p, const int32_t* __restrict__ state,
                                                           const uint8_t* __restrict__ done, int32_t* __restrict__ pool,
@@ -259,7 +260,7 @@ void launch_page_release(const PagePlan& p, const int32_t* state, const uint8_t*
 // out 16 bytes a feature, or in single values where the call does not fill an octet.  More features a workgroup leave
 // fewer of them on a CU to cover the two waits of each (slots, then rows): us at 512, 256 and 128 features 247, 184 and
 // 165 for the 17 s chunk, 92, 65 and 49 for the pieces.  Bound by HBM for many rows, where a large copy reaches 5.1 TB/s:
-// 105,462 rows of 8 heads of 64 150 us (4.3 TB/s), 8,700 rows of 32 and 8 heads of 128 45 us (4.5 TB/s); 62 rows 4.8 us,
+// 105,462 rows of 8 heads of 64 122 us (5.3 TB/s), 8,700 rows of 32 and 8 heads of 128 45 us (4.5 TB/s); 62 rows 4.8 us,
 // latency.
 constexpr int kAppendRows = 16, kAppendFeatures = 128;
 constexpr int kMostRows = 2 * kAppendRows - 1;            // rows of the groups that a tile writes
@@ -326,7 +327,8 @@ __global__ __launch_bounds__(256) void k_paged_append(AppendArgs a) {
   __shared__ int2 count;                 // rows and octets
   constexpr int kHead = D / 8;           // chunks of a head
   // A tile's parts run at the same time: its rows are read, and its groups written, in one go.  Workgroups are dealt to
-  // the 8 XCDs in turn, and parts that write K and V move twice what the others do: the parts start one later in each tile.
+  // the 8 XCDs in turn, and parts that write K and V move twice what the others do: the parts start one later in each tile
+  // (150 and 122 us for the 17 s chunk).
   const int tile = blockIdx.x / a.parts, row0 = tile * kAppendRows, lane = threadIdx.x & 63;
   const int part = int((blockIdx.x + tile) % uint32_t(a.parts));
   const bool is_q = part >= a.kv_parts;
