@@ -463,6 +463,30 @@ def test_attention_bounds_that_are_not_tight(hip):
         _attn_close(_run_attn(c, **kw), c)
 
 
+def test_attention_of_thousands_of_requests(hip):
+    """Column tiles found among 5000 requests: of no rows, of a few, of several tiles; of no positions."""
+    lens = [(37 * i) % 60 for i in range(5000)]
+    lens[0], lens[4100], lens[-1] = 300, 250, 140
+    new = [min(n, (13 * i) % 4) for i, n in enumerate(lens)]
+    new[0], new[4100], new[-1] = 200, 170, 140
+    c = _attn_case(lens, new, 2, 1, 64, 16, BF, 45, padding=3)
+    _say("attention of 5000 requests")
+    _attn_close(_run_attn(c, max_new=200, max_len=300), c)
+
+
+@pytest.mark.parametrize("R,max_new", [(5, 1), (5, 200), (64, 200), (65, 200)])
+def test_attention_of_starts_out_of_order_stays_in_its_rows(hip, R, max_new):
+    """starts that descend, are negative or pass the rows: what the rows get means nothing, and only rows are written."""
+    n, heads, D = 150, 2, 64
+    c = _attn_case([40 + i for i in range(R)], [0] * R, heads, 1, D, 16, BF, 46, padding=n)
+    c["starts"] = torch.randint(-100, 400, (R + 1,), generator=torch.Generator().manual_seed(R)).int()
+    c["starts"][:2] = _ints([-(1 << 31), (1 << 31) - 1])
+    room = torch.full((n + 64, heads * D), 7.0, dtype=BF, device=DEV)
+    _say("attention, starts out of order", R, max_new)
+    _run_attn(c, O=room[32:32 + n], max_new=max_new, max_len=100)
+    assert bool((room[:32] == 7.0).all()) and bool((room[32 + n:] == 7.0).all())
+
+
 def test_attention_is_the_same_bits_again_and_at_another_place_in_the_batch(hip):
     c = _attn_case([1500, 90, 700], [1, 1, 1], 4, 2, 64, 16, BF, 41)
     a = _run_attn(c, max_new=1)

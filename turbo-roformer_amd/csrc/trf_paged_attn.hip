@@ -107,7 +107,6 @@ __device__ __forceinline__ bool request_by_length(const Args& g, int t, int widt
   // keys (of 2^25 at most) and, for equal ones, the request: no two the same
   const int order = min(keys, (1 << 25) - 1) << 6 | (63 - lane);
   int first = 0;
-#pragma unroll 4
   for (int q = 0; q < R; ++q)
     first += __builtin_amdgcn_readlane(order, q) > order ? __builtin_amdgcn_readlane(tiles, q) : 0;
   const uint64_t found = __ballot(t >= first && t < first + tiles);

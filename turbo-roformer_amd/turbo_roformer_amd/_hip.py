@@ -738,7 +738,7 @@ def paged_attention(q, K, V, table, starts, lens, O, scale: float | None = None,
 
     ``scale``: None is head_dim ** -0.5; ``causal``: a row sees no later position; ``window`` > 0: only that many, up to
     its own; ``gate`` [n, heads] fp32.  ``max_new``, ``max_len``: bounds on the rows and the length of a request (None:
-    n, and what a table row holds): the tighter, the better the launch fits.  ``ws``: uint8 workspace of
+    n, and what a table row holds): the tighter, the better the launch fits; rows past ``max_new`` may be left out.  ``ws``: uint8 workspace of
     ``paged_attention_workspace_bytes`` (None: one from torch's allocator for this call)."""
     native, device, stream = _here()
     rc = native.paged_attention(device, stream, q, K, V, table, starts, lens, O, scale, causal, window, gate, max_new, max_len, ws)

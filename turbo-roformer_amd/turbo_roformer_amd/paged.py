@@ -75,7 +75,7 @@ class HipPagedCache:
 
     def plan(self, n_new: Tensor, rows: int, max_new: int | None = None) -> PageStep:
         """Deal pages for ``n_new`` [requests] int32 more rows of each request, ``rows`` of them in all or more (the rest is
-        padding); ``max_new``: a bound on a request's rows (None: ``rows``)."""
+        padding); ``max_new``: a bound on a request's rows (None: ``rows``), past which ``attend`` may leave rows out."""
         ints = dict(dtype=torch.int32, device=self.device)
         step = PageStep(torch.empty(self.table.shape[0] + 1, **ints), torch.empty(rows, **ints), torch.empty(rows, **ints),
                         rows if max_new is None else max_new)
