@@ -401,7 +401,8 @@ int trf_paged_append(const uint16_t* q, int64_t q_stride, int32_t heads, const u
                      int32_t n_pages, int32_t page_size, int32_t kv_heads, int32_t head_dim, uint16_t* q_out,
                      trf_stream_t stream);
 
-/* Workspace bytes of trf_paged_attention for these arguments (0: none is needed, or an argument is out of range). */
+/* Workspace bytes of trf_paged_attention for these arguments (0: none is needed, or an argument is out of range); a causal
+ * call or one with a window may need less. */
 size_t trf_paged_attention_workspace_bytes(int32_t heads, int32_t dtype, int32_t n_pages, int32_t page_size,
                                            int32_t kv_heads, int32_t head_dim, int32_t max_pages, int32_t n_requests,
                                            int32_t n_rows, int32_t max_new, int32_t max_len);

@@ -315,7 +315,7 @@ ATTN = [  # lens, new, heads, kv, page
     ([(37 * i) % 90 + 1 for i in range(70)], [min((37 * i) % 90 + 1, (13 * i) % 43) for i in range(70)], 4, 1, 16),
     ([200] * 5, [60, 3, 0, 45, 70], 4, 1, 32),
     # more than 1024 columns of a request
-    ([300, 40], [290, 3], 4, 1, 16), ([1100], [259], 8, 2, 64),
+    ([300, 40], [290, 3], 4, 1, 16), ([1100], [259], 8, 2, 64), ([600, 40], [290, 3], 4, 1, 32), ([1090, 1030], [1090, 3], 1, 1, 64),
 ]
 
 
@@ -327,7 +327,7 @@ def test_attention(hip, dtype, D, lens, new, heads, kv, page):
     _attn_close(_run_attn(c, max_new=max(new), max_len=max(lens)), c)
 
 
-@pytest.mark.parametrize("causal,window", [(True, 1), (True, 16), (True, 50), (True, 10_000), (False, 0), (False, 7), (False, 33)])
+@pytest.mark.parametrize("causal,window", [(True, 1), (True, 16), (True, 50), (True, 900), (True, 10_000), (False, 0), (False, 7), (False, 33)])
 @pytest.mark.parametrize("lens,new,page", [([200, 77], [1, 1], 16), ([150, 90], [40, 90], 32), ([333], [130], 64),
                                            ([2100, 90], [1, 1], 16), ([1300], [45], 64), ([310], [270], 32)])
 def test_attention_masks(hip, causal, window, lens, new, page):

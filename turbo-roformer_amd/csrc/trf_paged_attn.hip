@@ -790,15 +790,26 @@ Plan plan_of(const PagedShape& s, const PagedAttnArgs& a) {
   Plan p{};
   const int group = a.heads / s.kv_heads;
   const int64_t most = int64_t(a.max_new) * group;  // columns of a request, at most
-  // Two column tiles a wave for many columns: half the LDS reads, but the last tile of 256 and the keys of a causal one
-  // waste more. us for QT = 1 and 2, 62 sequences of 1701 with 8 heads of 64: 257 columns 89 and 126, 500 129 and 138, 900
-  // 212 and 223, 1701 278 and 288, not causal 436 and 413; 8 of 8000, 2048 columns 270 and 250.
-  p.qt = most <= kCols ? 0 : s.head_dim == 128 || most <= 1024 ? 1 : 2;
+  // keys that a row sees, at most
+  const int64_t keys = a.window ? std::min<int64_t>(a.max_len, int64_t(a.window) + (a.causal ? 0 : a.max_new)) : a.max_len;
+  // Two column tiles a wave for many columns: half the LDS reads, but the last tile of 256 and the keys of a causal one,
+  // whose rows end 256 / group keys apart, waste more. us for QT = 1 and 2, 62 sequences of 1701 with 8 heads of 64: 257
+  // columns 89 and 126, 500 129 and 138, 900 212 and 223, 1701 278 and 288, not causal 436 and 413; 62 of 1100, all their
+  // rows, 145 and 162, 10 of them 32 and 44; 8 of 8000, 2048 columns 270 and 250; 246 of 430, 412 rows of groups of 8 heads
+  // 265 and 247.
+  const bool two = most > 1024 && (!a.causal || keys * group > 2048);
+  p.qt = most <= kCols ? 0 : s.head_dim == 128 || !two ? 1 : 2;
   p.width = p.qt ? kWaves * kCols * p.qt : kCols;
   p.search = most > p.width;
   p.tiles = p.search ? int(int64_t(a.n_rows) * group / p.width) + a.n_requests : a.n_requests;
   const int64_t blocks = int64_t(p.tiles) * s.kv_heads, want = int64_t(device_cu_count()) * 2;
-  p.splits = int(std::min<int64_t>({want / blocks, a.max_len / 256, kMaxSplits}));
+  // A part has at least 256 of the keys that a tile's rows see, of many columns 128 up to one workgroup a CU: they have a
+  // longer way per key, but more partial sums to write (us at 256, 128 and this: one of 700 keys, 300 rows, 16 and 4 heads
+  // of 128 25, 18 and 18; four of them 27, 32 and 27; one of 1000 rows and keys, 8 heads of 64 14.3, 16.4 and 14.3).
+  const int64_t seen = std::min<int64_t>(a.max_len, keys + p.width / group);
+  int64_t parts = std::min(want / blocks, seen / 256);
+  if (p.qt) parts = std::max(parts, std::min(want / 2 / blocks, seen / 128));
+  p.splits = int(std::min<int64_t>(parts, kMaxSplits));
   if (p.splits < 3) p.splits = 1;
   // Requests by length where it matters: beyond some rounds of two workgroups a CU the last one is a small part of all.
   if (p.search && a.n_requests > 1 && a.n_requests <= 64 && blocks < 6 * want) p.search = 2;
@@ -807,6 +818,7 @@ Plan plan_of(const PagedShape& s, const PagedAttnArgs& a) {
 
 }  // namespace
 
+// No more for a causal call or one with a window than without.
 size_t paged_attention_workspace(const PagedShape& s, const PagedAttnArgs& a) {
   const Plan p = plan_of(s, a);
   return p.splits == 1 ? 0 : size_t(p.splits) * a.n_rows * a.heads * (s.head_dim + 2) * 4;

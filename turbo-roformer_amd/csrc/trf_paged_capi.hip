@@ -215,6 +215,8 @@ int trf_paged_attention(const uint16_t* q, int64_t q_stride, int32_t heads, cons
   TRF_REQUIRE_AT(lens, "lens", 4);
   if (gate) TRF_REQUIRE_AT(gate, "gate", 4);
   TRF_REQUIRE_AT(O, "O", 16);
+  a.causal = causal;
+  a.window = window;
   const size_t need = trf::paged_attention_workspace(s, a);
   if (need) {
     if (!workspace || workspace_bytes < need)
@@ -223,8 +225,6 @@ int trf_paged_attention(const uint16_t* q, int64_t q_stride, int32_t heads, cons
   }
   a.q = q, a.K = K, a.V = V, a.table = table, a.starts = starts, a.lens = lens, a.gate = gate, a.o = O;
   a.q_stride = q_stride;
-  a.causal = causal;
-  a.window = window;
   a.scale_log2 = scale * 1.44269504088896341f;
   trf::launch_paged_attention(s, a, workspace, as_hip(stream));
   return check_launch("paged_attention");
