@@ -1,5 +1,5 @@
 """The paged K/V cache in plain form: pages dealt request by request, rows written one by one, softmax by its
-definition in 64 bits.  Checker only; everything is on the CPU."""
+definition in 64 bits.  For tests only; everything is on the CPU."""
 
 from __future__ import annotations
 

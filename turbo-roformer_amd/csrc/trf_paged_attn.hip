@@ -468,8 +468,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void k_paged_attn_few
 //
 // Bound by the matrix pipe beside the softmax's vector work (about 50 instructions and 16 exponentials a step, for 10
 // (D = 64) or 18 MFMAs), and by the clock that the power limit leaves, 1.9-2.1 GHz.  Measured: 62 sequences of 1701 rows
-// over 1701 keys, 8 heads of 64, 412-447 us by host (820-890 TFLOP/s; a large library matrix product reaches 1190); 9
-// sequences of 300 to 600 rows over 2400 to 5800 keys, 32 and 8 heads of 128, 278-290 us (870 TFLOP/s: 1104 workgroups in
+// over 1701 keys, 8 heads of 64, 412-452 us by host (810-890 TFLOP/s; a large library matrix product reaches 1190); 9
+// sequences of 300 to 600 rows over 2400 to 5800 keys, 32 and 8 heads of 128, 278-292 us (830-870 TFLOP/s: 1104 workgroups in
 // 2.2 rounds of 512); 8 of 700 rows over 6000 keys 526 us (985 TFLOP/s).  Steps on the way (us for the first and the
 // second): K and V through LDS 566 and 371, three steps at once 521 and 344, two column tiles a wave and a loop without
 // edges 486 and 331.
