@@ -25,8 +25,6 @@ from pathlib import Path
 import numpy as np
 import torch
 
-sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "turbo-roformer_amd"))
-
 own = False
 
 DEV = "cuda"
@@ -228,6 +226,9 @@ def prepare(case: dict, seed: int) -> dict:
 def run(s: dict):
     kind = s["kind"]
     if own:
+        root = str(Path(__file__).resolve().parents[1] / "turbo-roformer_amd")
+        if root not in sys.path:
+            sys.path.insert(0, root)
         from turbo_roformer_amd import _hip
 
         if kind == "plan":
