@@ -18,6 +18,9 @@
 namespace trf {
 namespace {
 
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
 constexpr int kCols = 32;   // columns of an MFMA tile
 constexpr int kWaves = 4;   // waves of a workgroup
 // P may exceed 1 by this power of two before the running maximum is raised: fewer rescales, no loss (fp32 sums; P of
@@ -155,7 +158,7 @@ struct Acc {
   f32x16 o[D / 32];
   float m, shift;  // running maximum in the scores' own units, and times the scale (0 while there is none)
   float limit;     // scores above this raise it: kRaise past it, in the scores' own units
-  f32x4 sum;       // sums of P: column j < 16 in register 0 of lane j, column j + 16 in register 1 (row_sum)
+  f32x4 sum[2];    // this lane's sums of P's first and second halves of 8, in each register (row_sum)
 };
 
 template <int D>
@@ -165,7 +168,7 @@ __device__ __forceinline__ void clear(Acc<D>& s) {
   s.m = -INFINITY;
   s.limit = -INFINITY;
   s.shift = 0.f;
-  s.sum = f32x4{0.f, 0.f, 0.f, 0.f};
+  s.sum[0] = s.sum[1] = f32x4{0.f, 0.f, 0.f, 0.f};
 }
 
 // The keys that a column sees: lo .. lo + n - 1.
@@ -182,28 +185,33 @@ __device__ __forceinline__ Mask mask_of(const Args& g, const Tile& t, int col) {
 }
 
 // The sum of the rounded P, the weights that P.V applies, on the matrix pipe instead of by 16 additions a lane:
-// v_mfma_f32_16x16x32 takes P's registers as its B operand, whose lane l is column l % 16 and k-group l / 16; they hold
-// column l % 32 = l % 16 + 16 ((l / 16) & 1).  A's row 0 is 1 on k-groups 0 and 2, row 1 on 1 and 3, the rest 0.
+// v_mfma_f32_4x4x4 is 16 products of 4 x 4 matrices, lane l has column l % 4 of number l / 4, four values of it an
+// operand.  With ones for A each lane gets the sum of its own values, in all four registers: a NaN among them reaches no
+// other column, as it would with zeros in A (0 * NaN).  Two sums, so that no product waits for the one before it (the
+// 17 s chunk 436 us with one, 434 with two; v_mfma_f32_16x16x32 with zeros took 433).
 template <bool F16>
-__device__ __forceinline__ u32x4 sum_rows(int lane) {
-  const int m = lane & 15, k = (lane >> 4) & 1;
-  const uint32_t one = m == k && m < 2 ? (F16 ? 0x3c003c00u : 0x3f803f80u) : 0u;
-  return u32x4{one, one, one, one};
-}
-
-template <bool F16>
-__device__ __forceinline__ f32x4 row_sum(u32x4 ones, u32x4 p, f32x4 c) {
+__device__ __forceinline__ f32x4 sum4(uint32_t a, uint32_t b, f32x4 c) {
+  const u32x2 x{a, b}, ones = F16 ? u32x2{0x3c003c00u, 0x3c003c00u} : u32x2{0x3f803f80u, 0x3f803f80u};
   if constexpr (F16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, ones), __builtin_bit_cast(f16x8, p), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_4x4x4f16(__builtin_bit_cast(f16x4, ones), __builtin_bit_cast(f16x4, x), c, 0, 0, 0);
   else
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, ones), __builtin_bit_cast(bf16x8, p), c, 0,
-                                                   0, 0);
+    return __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(__builtin_bit_cast(s16x4, ones), __builtin_bit_cast(s16x4, x), c, 0, 0, 0);
 }
 
-// Column j's sum, j = lane % 32 (both halves get it).
-__device__ __forceinline__ float sum_of(const f32x4& sum, int j) {
-  const float a = __shfl(sum[0], j & 15), b = __shfl(sum[1], j & 15);
-  return j < 16 ? a : b;
+template <bool F16, int D>
+__device__ __forceinline__ void row_sum(Acc<D>& acc, u32x4 p0, u32x4 p1) {
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    acc.sum[0] = sum4<F16>(p0[i], p0[i + 1], acc.sum[0]);
+    acc.sum[1] = sum4<F16>(p1[i], p1[i + 1], acc.sum[1]);
+  }
+}
+
+// A column's sum, of its two lanes.
+template <int D>
+__device__ __forceinline__ float sum_of(const Acc<D>& acc) {
+  const float l = acc.sum[0][0] + acc.sum[1][0];
+  return l + __shfl_xor(l, 32);
 }
 
 // The largest score of this lane's half of a column.
@@ -222,7 +230,7 @@ __device__ __forceinline__ bool above(const Acc<D>& acc, float top) {
 
 // Raises the maxima of the columns that are.
 template <int D>
-__device__ __forceinline__ void raise(Acc<D>& acc, float half_top, float c, int lane) {
+__device__ __forceinline__ void raise(Acc<D>& acc, float half_top, float c) {
   const float top = halfwave_max(half_top);
   const bool up = top > acc.limit;
   const float f = up ? __builtin_amdgcn_exp2f((acc.m - top) * c) : 1.f;
@@ -236,7 +244,7 @@ __device__ __forceinline__ void raise(Acc<D>& acc, float half_top, float c, int 
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc.o[d][r] *= f;
   acc.sum[0] *= f;
-  acc.sum[1] *= __shfl(f, (lane & 15) + 16);
+  acc.sum[1] *= f;
 }
 
 // Half of a tile's scores -> P as a B operand: rounded to the type of V, as the matrix instruction takes both in one type.
@@ -288,7 +296,7 @@ __device__ __forceinline__ void load_q(const Args& g, const Tile& t, int col, in
 }
 
 // Columns' rows out: four features of a column, divided by its sum and gated; zeros for a row that saw no key, whose sum
-// is zero (by its bits: a NaN is not).
+// is zero (where it is NaN so is o, and stays it).
 template <int D, bool F16>
 __device__ __forceinline__ void store4(const Args& g, int64_t out, int quad, const f32x4& o, float l) {
   const float f = __float_as_uint(l) << 1 ? (g.a.gate ? g.a.gate[out] : 1.f) / l : 0.f;
@@ -335,7 +343,6 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void k_paged_attn_few
   const Mask mask = mask_of(g, t, col);
   Acc<D> acc;
   clear(acc);
-  const u32x4 ones = sum_rows<F16>(lane);
   const float c = g.a.scale_log2;
   const int32_t* table = g.a.table + int64_t(t.r) * g.a.max_pages;
   const uint32_t page_bytes = uint32_t(g.kv_heads) * D * 2 << g.page_shift;
@@ -385,9 +392,9 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void k_paged_attn_few
           for (int i = 0; i < 4; ++i) x.va[d][u][i] = finite2<F16>(x.va[d][u][i], odd);
     }
     const float top = half_max(s);
-    if (above(acc, top)) raise(acc, top, c, lane);
+    if (above(acc, top)) raise(acc, top, c);
     const u32x4 p0 = weights<F16, 0>(s, c, acc.shift), p1 = weights<F16, 1>(s, c, acc.shift);
-    acc.sum = row_sum<F16>(ones, p1, row_sum<F16>(ones, p0, acc.sum));
+    row_sum<F16>(acc, p0, p1);
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       acc.o[d] = mfma<F16>(x.va[d][0], p0, acc.o[d]);
@@ -418,7 +425,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void k_paged_attn_few
     if (kt + 2 * kWaves < k1) load(even, kt + 2 * kWaves);
     compute(odd, kt + kWaves);
   }
-  const float l = sum_of(acc.sum, j);
+  const float l = sum_of(acc);
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -466,8 +473,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void k_paged_attn_few
 // take turns on the two column tiles, and each K and V operand read from LDS feeds two products.  Raising the maximum,
 // masks and infinities leave that path (rare).
 //
-// Bound by the matrix pipe beside the softmax's vector work (about 50 instructions and 16 exponentials a step, for 10
-// (D = 64) or 18 MFMAs), and by the clock that the power limit leaves, 1.9-2.1 GHz.  Measured: 62 sequences of 1701 rows
+// Bound by the matrix pipe beside the softmax's vector work (about 50 instructions and 16 exponentials a step, for 12
+// (D = 64) or 20 MFMAs, 4 of them small), and by the clock that the power limit leaves, 1.9-2.1 GHz.  Measured: 62 sequences of 1701 rows
 // over 1701 keys, 8 heads of 64, 412-452 us by host (810-890 TFLOP/s; a large library matrix product reaches 1190); 9
 // sequences of 300 to 600 rows over 2400 to 5800 keys, 32 and 8 heads of 128, 278-292 us (830-870 TFLOP/s: 1104 workgroups in
 // 2.2 rounds of 512); 8 of 700 rows over 6000 keys 526 us (985 TFLOP/s).  Steps on the way (us for the first and the
@@ -551,7 +558,6 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && QT == 1 ? 3 : 2) void k_pag
     mask[x] = mask_of(g, t, col0 + kCols * x + j);
     clear(acc[x]);
   }
-  const u32x4 ones = sum_rows<F16>(lane);
 
   // places of units in the ring
   const int k_lane = (j >> 4) * M::kGroup + hh * 16 + key_slot(j & 15);
@@ -641,7 +647,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && QT == 1 ? 3 : 2) void k_pag
           p_v(x);
           no_p_v();
         }
-        raise(acc[x], top, c, lane);
+        raise(acc[x], top, c);
       }
       // two stretches of matrix work with vector work of about its length, and the operands' loads behind each
       scores(s_next, last ? 0 : x + 1);
@@ -652,7 +658,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && QT == 1 ? 3 : 2) void k_pag
       p1[x] = weights<F16, 1>(s, c, acc[x].shift);
       p0[x] = n0;
       __builtin_amdgcn_sched_barrier(0);
-      acc[x].sum = row_sum<F16>(ones, p1[x], row_sum<F16>(ones, p0[x], acc[x].sum));
+      row_sum<F16>(acc[x], p0[x], p1[x]);
       if (QT == 1) {  // K first: the next step begins with it
         advance(i);
         load_k(after(at1, i + 2));
@@ -720,7 +726,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && QT == 1 ? 3 : 2) void k_pag
 #pragma unroll
   for (int x = 0; x < QT; ++x) {
     const int col = col0 + kCols * x + j;
-    const float l = sum_of(acc[x].sum, j);
+    const float l = sum_of(acc[x]);
     if (col >= t.cols) continue;
     const int64_t out = out_row(g, t, col), part = int64_t(blockIdx.y) * g.a.n_rows * g.a.heads + out;
 #pragma unroll
