@@ -382,6 +382,13 @@ int trf_page_plan(const int32_t* state, const int32_t* n_new, int32_t n_requests
                   int32_t n_pages, int32_t page_size, int32_t* table, int32_t max_pages, int32_t* state_out,
                   int32_t* starts, int32_t* slots, int32_t* positions, trf_stream_t stream);
 
+/* The same with requests of at most max_length positions, 1 .. max_pages * page_size: one whose length would pass that
+ * is refused, though its last page has room. */
+int trf_page_plan_limited(const int32_t* state, const int32_t* n_new, int32_t n_requests, int32_t n_rows,
+                          const int32_t* pool, int32_t n_pages, int32_t page_size, int32_t* table, int32_t max_pages,
+                          int32_t max_length, int32_t* state_out, int32_t* starts, int32_t* slots, int32_t* positions,
+                          trf_stream_t stream);
+
 /* Give the pages of the requests with done[r] != 0 back: the ceil(len / page_size) first entries of their table
  * rows go to the pool from entry state[0] on, in the order of requests and positions; state_out holds the new count
  * of free pages, 0 refused requests and the lengths, 0 for these requests.  table is left as it is. */

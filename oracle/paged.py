@@ -10,9 +10,10 @@ import torch
 Tensor = torch.Tensor
 
 
-def plan(state, n_new, pool, table, page: int, n_rows: int) -> dict[str, Tensor]:
-    """The deal of ``trf_page_plan``: state_out, starts, slots, positions and table (a copy)."""
+def plan(state, n_new, pool, table, page: int, n_rows: int, max_length: int | None = None) -> dict[str, Tensor]:
+    """The deal of ``trf_page_plan_limited``: state_out, starts, slots, positions and table (a copy)."""
     R, max_pages = table.shape
+    longest = max_pages * page if max_length is None else max_length
     n_pages = pool.numel()
     table = table.clone()
     free = min(max(int(state[0]), 0), n_pages)
@@ -22,7 +23,7 @@ def plan(state, n_new, pool, table, page: int, n_rows: int) -> dict[str, Tensor]
     for r in range(R):
         n, length = max(int(n_new[r]), 0), min(max(int(state[2 + r]), 0), max_pages * page)
         have, need = -(-length // page), -(-(length + n) // page)
-        fits = row + n <= n_rows and length + n <= max_pages * page
+        fits = row + n <= n_rows and length + n <= longest
         owed += need - have if fits else 0
         if fits and (need == have or owed <= free):
             for j in range(have, need):

@@ -204,6 +204,7 @@ constexpr int kPageRequests = 8192;
 
 struct PagePlan {
   int32_t n_requests, n_rows, n_pages, page_shift, max_pages;  // page_shift: log2 of the page size
+  int32_t max_length;  // of a request that takes new rows, at most max_pages pages
 };
 
 // K [n_pages][kv_heads][page / 16][head_dim / 8][16][8], V [n_pages][kv_heads][page / 8][head_dim][8]: the 16

@@ -93,6 +93,18 @@ int trf_page_plan(const int32_t* state, const int32_t* n_new, int32_t n_requests
                   int32_t* starts, int32_t* slots, int32_t* positions, trf_stream_t stream) {
   TRF_TRY(check_pages(n_pages, page_size));
   TRF_TRY(check_table(n_requests, max_pages, page_size));
+  return trf_page_plan_limited(state, n_new, n_requests, n_rows, pool, n_pages, page_size, table, max_pages,
+                               max_pages * page_size, state_out, starts, slots, positions, stream);
+}
+
+int trf_page_plan_limited(const int32_t* state, const int32_t* n_new, int32_t n_requests, int32_t n_rows,
+                          const int32_t* pool, int32_t n_pages, int32_t page_size, int32_t* table, int32_t max_pages,
+                          int32_t max_length, int32_t* state_out, int32_t* starts, int32_t* slots, int32_t* positions,
+                          trf_stream_t stream) {
+  TRF_TRY(check_pages(n_pages, page_size));
+  TRF_TRY(check_table(n_requests, max_pages, page_size));
+  if (max_length < 1 || max_length > max_pages * page_size)
+    return set_error(TRF_ERR_ARG, "max_length must be 1..%d, got %d", max_pages * page_size, max_length);
   if (n_requests > trf::kPageRequests)
     return set_error(TRF_ERR_ARG, "n_requests must be at most %d, got %d", trf::kPageRequests, n_requests);
   if (n_rows < 0 || n_rows >= 1 << 30) return set_error(TRF_ERR_ARG, "n_rows must be 0..2^30 - 1, got %d", n_rows);
@@ -105,7 +117,7 @@ int trf_page_plan(const int32_t* state, const int32_t* n_new, int32_t n_requests
     TRF_REQUIRE_AT(slots, "slots", 4);
     TRF_REQUIRE_AT(positions, "positions", 4);
   }
-  const trf::PagePlan p{n_requests, n_rows, n_pages, page_shift(page_size), max_pages};
+  const trf::PagePlan p{n_requests, n_rows, n_pages, page_shift(page_size), max_pages, max_length};
   trf::launch_page_plan(p, state, n_new, pool, table, state_out, starts, slots, positions, as_hip(stream));
   return check_launch("page_plan");
 }
@@ -120,7 +132,7 @@ int trf_page_release(const int32_t* state, const uint8_t* done, int32_t n_reques
   TRF_REQUIRE_AT(done, "done", 1);
   TRF_REQUIRE_AT(pool, "pool", 4);
   TRF_REQUIRE_AT(table, "table", 4);
-  const trf::PagePlan p{n_requests, 0, n_pages, page_shift(page_size), max_pages};
+  const trf::PagePlan p{n_requests, 0, n_pages, page_shift(page_size), max_pages, max_pages * page_size};
   trf::launch_page_release(p, state, done, pool, table, state_out, as_hip(stream));
   return check_launch("page_release");
 }

@@ -98,12 +98,11 @@ __global__ __launch_bounds__(THREADS) void k_page_plan(PagePlan p, const int32_t
   }
   const int free = min(max(state[0], 0), p.n_pages);
   // Pages are wanted by requests whose rows fit; that they all do is what both sums are formed on at once.
-  const int64_t cap = int64_t(p.max_pages) << p.page_shift;
   uint32_t want[EACH], want_mine = 0;
   bool fits[EACH];
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
-    fits[e] = r0 + e < R && int64_t(len[e]) + n[e] <= cap;
+    fits[e] = r0 + e < R && int64_t(len[e]) + n[e] <= p.max_length;
     want[e] = fits[e] ? ((len[e] + n[e] + page - 1) >> p.page_shift) - ((len[e] + page - 1) >> p.page_shift) : 0;
     want_mine += want[e];
     mine = min(mine + n[e], beyond);

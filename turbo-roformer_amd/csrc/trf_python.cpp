@@ -7,6 +7,7 @@
 // returns the C ABI's status.  ValueError: a tensor does not fit; TypeError: something is no tensor.
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <stdexcept>
 
@@ -14,7 +15,7 @@
 
 namespace {
 
-decltype(&trf_page_plan) page_plan_fn;
+decltype(&trf_page_plan_limited) page_plan_fn;
 decltype(&trf_page_release) page_release_fn;
 decltype(&trf_paged_append) paged_append_fn;
 decltype(&trf_paged_attention) paged_attention_fn;
@@ -148,8 +149,9 @@ int unlocked(F f) {
   return rc;
 }
 
+// max_length may be left out: as long as the table's rows.
 PyObject* page_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return call(a, n, 11, [](Args& x, trf_stream_t stream) {
+  return call(a, n, n == 12 ? 12 : 11, [n](Args& x, trf_stream_t stream) {
     const at::Tensor &state = *x.tensor("state"), &n_new = *x.tensor("n_new"), &pool = *x.tensor("pool"), &table = *x.tensor("table");
     const int32_t page_size = x.number32("page_size"), R = length(table, "table", 2, 0), max_pages = length(table, "table", 2, 1);
     const int32_t pages = length(pool, "pool", 1, 0);
@@ -163,9 +165,10 @@ PyObject* page_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int32_t rows = length(slots, "slots", 1, 0);
     need(slots, "slots", at::kInt, {rows});
     int32_t* positions = ints(x, "positions", {rows});
+    const int32_t longest = n == 12 ? x.number32("max_length") : int32_t(std::min<int64_t>(int64_t(max_pages) * page_size, INT32_MAX));
     return unlocked([&] {
       return page_plan_fn(address<int32_t>(&state), address<int32_t>(&n_new), R, rows, address<int32_t>(&pool), pages, page_size,
-                          address<int32_t>(&table), max_pages, out, starts, address<int32_t>(&slots), positions, stream);
+                          address<int32_t>(&table), max_pages, longest, out, starts, address<int32_t>(&slots), positions, stream);
     });
   });
 }
@@ -274,8 +277,9 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(name)), METH_FASTCALL, doc}
 
 PyMethodDef methods[] = {
-    TRF_METHOD(bind, "bind(page_plan, page_release, paged_append, paged_attention): the C functions' addresses"),
-    TRF_METHOD(page_plan, "page_plan(device, stream, state, n_new, pool, table, page_size, state_out, starts, slots, positions)"),
+    TRF_METHOD(bind, "bind(page_plan_limited, page_release, paged_append, paged_attention): the C functions' addresses"),
+    TRF_METHOD(page_plan,
+               "page_plan(device, stream, state, n_new, pool, table, page_size, state_out, starts, slots, positions[, max_length])"),
     TRF_METHOD(page_release, "page_release(device, stream, state, done, pool, table, page_size, state_out)"),
     TRF_METHOD(paged_append, "paged_append(device, stream, k, v, K, V, slots, positions, rope, q, q_out)"),
     TRF_METHOD(paged_attention,

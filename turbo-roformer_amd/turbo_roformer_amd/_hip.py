@@ -117,6 +117,7 @@ _SIGNATURES: dict[str, tuple] = {
     ),
     "trf_mask_head": (ctypes.c_int, [_P, _I32, _I32, ctypes.POINTER(ctypes.c_int32), _I32, _P, _I32, _P, _P]),
     "trf_page_plan": (ctypes.c_int, [_P, _P, _I32, _I32, _P, _I32, _I32, _P, _I32, _P, _P, _P, _P, _P]),
+    "trf_page_plan_limited": (ctypes.c_int, [_P, _P, _I32, _I32, _P, _I32, _I32, _P, _I32, _I32, _P, _P, _P, _P, _P]),
     "trf_page_release": (ctypes.c_int, [_P, _P, _I32, _P, _I32, _I32, _P, _I32, _P, _P]),
     "trf_paged_append": (
         ctypes.c_int,
@@ -189,7 +190,7 @@ def bind_native(lib: ctypes.CDLL):
         from . import _native as native
     except ImportError as e:
         raise HipUnavailable(f"_native.so cannot be loaded ({e}): run `make -C turbo-roformer_amd/csrc`") from None
-    names = ("trf_page_plan", "trf_page_release", "trf_paged_append", "trf_paged_attention")
+    names = ("trf_page_plan_limited", "trf_page_release", "trf_paged_append", "trf_paged_attention")
     native.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names))
     _native = native
     return native
@@ -700,13 +701,15 @@ def paged_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, dtype:
     return K, V
 
 
-def page_plan(state, n_new, pool, table, page_size: int, state_out, starts, slots, positions) -> None:
+def page_plan(state, n_new, pool, table, page_size: int, state_out, starts, slots, positions,
+              max_length: int | None = None) -> None:
     """Deal pages for ``n_new`` [R] more rows of each request and say where they go (``trf_page_plan``): ``state`` [2 + R]
     (free pages, refused requests, lengths) -> ``state_out``, ``table`` [R, max pages] in place, ``starts`` [R + 1],
     and for each of the rows that ``slots`` and ``positions`` have room for its slot and position, -1 where there
-    is none.  All int32 on the device."""
+    is none.  All int32 on the device.  ``max_length``: longer requests are refused (None: ones longer than a table row)."""
     native, device, stream = _here()
-    rc = native.page_plan(device, stream, state, n_new, pool, table, page_size, state_out, starts, slots, positions)
+    limit = () if max_length is None else (max_length,)
+    rc = native.page_plan(device, stream, state, n_new, pool, table, page_size, state_out, starts, slots, positions, *limit)
     if rc:
         _check(rc)
 

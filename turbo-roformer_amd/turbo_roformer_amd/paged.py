@@ -49,6 +49,7 @@ class HipPagedCache:
         _hip.load()
         self.device = torch.device(device)
         self.page_size = page_size
+        self.max_length = max_length
         self.max_pages = -(-max_length // page_size) if page_size > 0 else 0
         self.pages = requests * self.max_pages if pages is None else pages
         self.K, self.V = _hip.paged_cache(self.pages, page_size, kv_heads, head_dim, dtype, self.device)
@@ -80,13 +81,15 @@ class HipPagedCache:
         step = PageStep(torch.empty(self.table.shape[0] + 1, **ints), torch.empty(rows, **ints), torch.empty(rows, **ints),
                         rows if max_new is None else max_new)
         _hip.page_plan(self.state, n_new, self.pool, self.table, self.page_size, self._next, step.starts, step.slots,
-                       step.positions)
+                       step.positions, self.max_length)
         self.state.copy_(self._next)
         return step
 
     def append(self, step: PageStep, q: Tensor | None, k: Tensor, v: Tensor, rope: Tensor | None = None) -> Tensor | None:
-        """Write the step's rows k and v [rows, kv heads, head dim] to the cache, k rotated by ``rope`` [2, P, head dim / 2];
-        returns q [rows, heads, head dim] rotated (rows without a place are not written)."""
+        """Write the step's rows k and v [rows, kv heads, head dim] to the cache, k rotated by ``rope`` [2, P, head dim / 2]
+        with P at least ``max_length``; returns q [rows, heads, head dim] rotated (rows without a place are not written)."""
+        if rope is not None and rope.dim() == 3 and rope.shape[1] < self.max_length:
+            raise ValueError(f"rope has {rope.shape[1]} positions, the cache's requests have up to {self.max_length}")
         out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
         _hip.paged_append(k, v, self.K, self.V, step.slots, step.positions, rope, q, out)
         return out
