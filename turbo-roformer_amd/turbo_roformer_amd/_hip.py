@@ -177,9 +177,7 @@ def load() -> ctypes.CDLL:
         if not ok:
             raise HipUnavailable(reason)
         torch.cuda.init()  # the library must bind to torch's HIP runtime, loaded first
-        lib = open_library()
-        bind_native(lib)
-        _lib = lib
+        _lib = open_library()
         return _lib
 
 
@@ -194,6 +192,11 @@ def bind_native(lib: ctypes.CDLL):
     native.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names))
     _native = native
     return native
+
+
+def load_native():
+    """The bound module; only the paged cache's entry points need it.  Raises HipUnavailable."""
+    return _native if _native is not None else bind_native(load())
 
 
 def is_loaded() -> bool:
@@ -667,10 +670,9 @@ def overlap_finish(acc: torch.Tensor, wsum: torch.Tensor, gain: float, out: torc
 
 def _here() -> tuple:
     """The module of the entry points, the current device and its current stream."""
-    if _native is None:
-        load()
+    native = load_native()
     device = torch.cuda.current_device()
-    return _native, device, torch._C._cuda_getCurrentRawStream(device)  # current_stream() makes an object first, a us
+    return native, device, torch._C._cuda_getCurrentRawStream(device)  # current_stream() makes an object first, a us
 
 
 def _cache(K: torch.Tensor, V: torch.Tensor) -> tuple[int, int, int, int, int]:

@@ -46,7 +46,7 @@ class HipPagedCache:
                  device: str | torch.device = "cuda"):
         if requests < 1 or max_length < 1:
             raise ValueError(f"requests and max_length must be >= 1, got {requests} and {max_length}")
-        _hip.load()
+        _hip.load_native()
         self.device = torch.device(device)
         self.page_size = page_size
         self.max_length = max_length
