@@ -3,6 +3,8 @@
 from __future__ import annotations
 
 import sys
+import sysconfig
+import types
 
 import pytest
 import torch
@@ -45,3 +47,24 @@ def test_it_is_bound_at_the_first_paged_call(unloaded):
     assert _hip._native is None
     HipPagedCache(2, 64, device="cpu")
     assert _hip._native is not None
+
+
+def test_its_name_carries_the_pythons_tag():
+    native = _hip.bind_native(_hip.open_library())
+    assert native.__file__.endswith(sysconfig.get_config_var("EXT_SUFFIX"))
+
+
+@pytest.mark.parametrize("attributes", [{}, dict(abi_version=_hip.ABI_VERSION), dict(abi_version=_hip.ABI_VERSION - 1, functions=("trf_page_plan",) * 4),
+                                        dict(abi_version=_hip.ABI_VERSION, functions=("trf_page_plan", "trf_no_such_function"))])
+def test_a_module_of_another_library_is_not_bound(monkeypatch, attributes):
+    """One that takes functions this library does not have, or has with other arguments."""
+    lib = _hip.open_library()
+    other = types.ModuleType("turbo_roformer_amd._native")
+    other.bind = lambda *addresses: pytest.fail("bound")
+    vars(other).update(attributes)
+    monkeypatch.setattr(turbo_roformer_amd, "_native", other, raising=False)
+    monkeypatch.setitem(sys.modules, "turbo_roformer_amd._native", other)
+    monkeypatch.setattr(_hip, "_native", None)
+    with pytest.raises(_hip.HipUnavailable, match="not of this library"):
+        _hip.bind_native(lib)
+    assert _hip._native is None

@@ -290,4 +290,13 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods};
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__native() { return PyModule_Create(&module); }
+// abi_version: of the header that this was compiled with.  functions: what bind() wants the addresses of, in its order.
+PyMODINIT_FUNC PyInit__native() {
+  PyObject* m = PyModule_Create(&module);
+  PyObject* names = Py_BuildValue("(ssss)", "trf_page_plan_limited", "trf_page_release", "trf_paged_append", "trf_paged_attention");
+  if (m && names && PyModule_AddIntConstant(m, "abi_version", TRF_ABI_VERSION) == 0 && PyModule_AddObject(m, "functions", names) == 0)
+    return m;
+  Py_XDECREF(names);
+  Py_XDECREF(m);
+  return nullptr;
+}

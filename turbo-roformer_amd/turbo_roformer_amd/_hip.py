@@ -187,8 +187,11 @@ def bind_native(lib: ctypes.CDLL):
     try:
         from . import _native as native
     except ImportError as e:
-        raise HipUnavailable(f"_native.so cannot be loaded ({e}): run `make -C turbo-roformer_amd/csrc`") from None
-    names = ("trf_page_plan_limited", "trf_page_release", "trf_paged_append", "trf_paged_attention")
+        raise HipUnavailable(f"the module _native cannot be loaded ({e}): run `make -C turbo-roformer_amd/csrc native`") from None
+    version, names = getattr(native, "abi_version", None), getattr(native, "functions", ())
+    if version != lib.trf_abi_version() or not names or any(n not in _SIGNATURES for n in names):
+        raise HipUnavailable(f"the module _native is not of this library (ABI version {version} and {lib.trf_abi_version()}): "
+                             "run `make -C turbo-roformer_amd/csrc native`")
     native.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names))
     _native = native
     return native
