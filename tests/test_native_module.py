@@ -2,9 +2,11 @@
 
 from __future__ import annotations
 
+import subprocess
 import sys
 import sysconfig
 import types
+from pathlib import Path
 
 import pytest
 import torch
@@ -68,3 +70,10 @@ def test_a_module_of_another_library_is_not_bound(monkeypatch, attributes):
     with pytest.raises(_hip.HipUnavailable, match="not of this library"):
         _hip.bind_native(lib)
     assert _hip._native is None
+
+
+def test_the_library_builds_without_python():
+    """Its makefile's default target names no file of the module."""
+    csrc = Path(__file__).resolve().parents[1] / "turbo-roformer_amd" / "csrc"
+    plan = subprocess.run(["make", "-n", "-B", "-C", str(csrc), "PYTHON=/no/such/python"], capture_output=True, text=True, check=True)
+    assert "libtrf_hip.so" in plan.stdout and "trf_python.cpp" not in plan.stdout
