@@ -85,3 +85,16 @@ def test_plan_within_a_length(hip, R, page, most):
     for longest in (-1, table.shape[1] * page + 1):
         with pytest.raises(RuntimeError, match="max_length"):
             _hip.page_plan(*dev, page, *out, max_length=longest)
+
+
+def test_refused_is_the_last_plans_after_a_release(hip):
+    """A step reads it at its end, where it can wait for the device."""
+    cache = HipPagedCache(3, 64, 1, 64, pages=3, page_size=16)
+    assert cache.refused == 0
+    cache.plan(_ints([16, 20, 5]).to(DEV), 41)
+    cache.release(torch.tensor([True, False, False], device=DEV))
+    assert cache.refused == 1 and cache.lengths.tolist() == [0, 20, 0] and cache.free_pages == 1
+    cache.release(torch.tensor([False, True, False], device=DEV))
+    assert cache.refused == 1 and cache.lengths.tolist() == [0, 0, 0] and cache.free_pages == 3
+    cache.plan(_ints([0, 0, 5]).to(DEV), 5)
+    assert cache.refused == 0

@@ -57,7 +57,7 @@ class HipPagedCache:
         self.pool = torch.arange(self.pages, dtype=torch.int32, device=self.device)
         self.state = torch.zeros(2 + requests, dtype=torch.int32, device=self.device)
         self.state[:1] = self.pages
-        self._next = torch.empty_like(self.state)
+        self._planned, self._released = torch.zeros_like(self.state), torch.zeros_like(self.state)
 
     @property
     def lengths(self) -> Tensor:
@@ -71,8 +71,9 @@ class HipPagedCache:
 
     @property
     def refused(self) -> int:
-        """Requests that the last ``plan`` refused, for want of pages, of rows or of length (waits for the device)."""
-        return int(self.state[1])
+        """Requests that the last ``plan`` refused, for want of pages, of rows or of length (waits for the device); a
+        ``release`` since then does not change it."""
+        return int(self._planned[1])
 
     def plan(self, n_new: Tensor, rows: int, max_new: int | None = None) -> PageStep:
         """Deal pages for ``n_new`` [requests] int32 more rows of each request, ``rows`` of them in all or more (the rest is
@@ -80,9 +81,9 @@ class HipPagedCache:
         ints = dict(dtype=torch.int32, device=self.device)
         step = PageStep(torch.empty(self.table.shape[0] + 1, **ints), torch.empty(rows, **ints), torch.empty(rows, **ints),
                         rows if max_new is None else max_new)
-        _hip.page_plan(self.state, n_new, self.pool, self.table, self.page_size, self._next, step.starts, step.slots,
+        _hip.page_plan(self.state, n_new, self.pool, self.table, self.page_size, self._planned, step.starts, step.slots,
                        step.positions, self.max_length)
-        self.state.copy_(self._next)
+        self.state.copy_(self._planned)
         return step
 
     def append(self, step: PageStep, q: Tensor | None, k: Tensor, v: Tensor, rope: Tensor | None = None) -> Tensor | None:
@@ -106,5 +107,5 @@ class HipPagedCache:
 
     def release(self, done: Tensor) -> None:
         """Take the pages of the requests with ``done`` [requests] (bool) back; their lengths become 0."""
-        _hip.page_release(self.state, done, self.pool, self.table, self.page_size, self._next)
-        self.state.copy_(self._next)
+        _hip.page_release(self.state, done, self.pool, self.table, self.page_size, self._released)
+        self.state.copy_(self._released)
