@@ -424,7 +424,8 @@ size_t trf_paged_attention_workspace_bytes(int32_t heads, int32_t dtype, int32_t
  * max_new and max_len are the caller's bounds on the rows and the length of a request, from which the launch is
  * chosen: rows past max_new may be left out, max_len bounds nothing but speed.  n_rows * heads is below 2^31, and
  * (n_rows * heads / kv_heads / 32 + n_requests) * kv_heads below 2^24.  P is rounded to the dtype for P V,
- * unnormalised; scores, their maximum and the sums are fp32.  The same call gives the same bits.
+ * unnormalised (in fp16 weights of less than 2^-32 of the largest count as none); scores, their maximum and the sums
+ * are fp32, which holds scale * q.k up to 2^24.  The same call gives the same bits.
  * workspace: trf_paged_attention_workspace_bytes, 16-byte aligned, of any content, in use until the call's work is
  * done: calls that may overlap need one each. */
 int trf_paged_attention(const uint16_t* q, int64_t q_stride, int32_t heads, const uint16_t* K, const uint16_t* V,

@@ -23,9 +23,15 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kCols = 32;   // columns of an MFMA tile
 constexpr int kWaves = 4;   // waves of a workgroup
-// P may exceed 1 by this power of two before the running maximum is raised: fewer rescales, no loss (fp32 sums; P of
-// at most 256 is well inside fp16).
+// P may exceed its value at the running maximum by this power of two before that is raised: fewer rescales, no loss (fp32
+// sums).  fp16 reaches from 2^-24 to 2^16: there P is 2^7 at the maximum, so that it keeps to 2^15 and weights down to
+// 2^-31 of the largest are not lost (of 131,071 keys with 2^-26 of it each, together 2^-9 of the sum, nothing was left).
 constexpr float kRaise = 8.0f;
+template <bool F16>
+constexpr float kAtMax = F16 ? 7.0f : 0.0f;
+// What the shift and the limit are rounded by grows with the scores: past this, times the scale, every larger one raises
+// the maximum.
+constexpr float kLargeScore = 4194304.0f;
 
 struct Args {
   PagedAttnArgs a;
@@ -156,7 +162,7 @@ __device__ __forceinline__ bool find_tile(const Args& g, int tile, int h, int wi
 template <int D>
 struct Acc {
   f32x16 o[D / 32];
-  float m, shift;  // running maximum in the scores' own units, and times the scale (0 while there is none)
+  float m, shift;  // running maximum in the scores' own units, and times the scale, less kAtMax (0 while there is none)
   float limit;     // scores above this raise it: kRaise past it, in the scores' own units
   f32x4 sum[2];    // this lane's sums of P's first and second halves of 8, in each register (row_sum)
 };
@@ -229,15 +235,15 @@ __device__ __forceinline__ bool above(const Acc<D>& acc, float top) {
 }
 
 // Raises the maxima of the columns that are.
-template <int D>
+template <bool F16, int D>
 __device__ __forceinline__ void raise(Acc<D>& acc, float half_top, float c) {
   const float top = halfwave_max(half_top);
   const bool up = top > acc.limit;
   const float f = up ? __builtin_amdgcn_exp2f((acc.m - top) * c) : 1.f;
   if (up) {
     acc.m = top;
-    acc.shift = top * c;
-    acc.limit = top + kRaise / c;
+    acc.shift = top * c - kAtMax<F16>;
+    acc.limit = fabsf(acc.shift) < kLargeScore ? top + kRaise / c : top;
   }
 #pragma unroll
   for (int d = 0; d < D / 32; ++d)
@@ -392,7 +398,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void k_paged_attn_few
           for (int i = 0; i < 4; ++i) x.va[d][u][i] = finite2<F16>(x.va[d][u][i], odd);
     }
     const float top = half_max(s);
-    if (above(acc, top)) raise(acc, top, c);
+    if (above(acc, top)) raise<F16>(acc, top, c);
     const u32x4 p0 = weights<F16, 0>(s, c, acc.shift), p1 = weights<F16, 1>(s, c, acc.shift);
     row_sum<F16>(acc, p0, p1);
 #pragma unroll
@@ -647,7 +653,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && QT == 1 ? 3 : 2) void k_pag
           p_v(x);
           no_p_v();
         }
-        raise(acc[x], top, c);
+        raise<F16>(acc[x], top, c);
       }
       // two stretches of matrix work with vector work of about its length, and the operands' loads behind each
       scores(s_next, last ? 0 : x + 1);
