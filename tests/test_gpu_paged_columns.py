@@ -91,3 +91,12 @@ def test_thirty_two_parts(hip, dtype, D, lens, new, heads, page):
     _say("32 parts", dtype, D, lens, new)
     _attn_close(_run_attn(c, max_new=max(new), max_len=max(lens)), c)
 
+
+
+@pytest.mark.parametrize("D", (64, 128))
+def test_entries_that_are_no_pages_in_some_of_the_parts(hip, D):
+    """Each part of the keys looks at the table entries of its own keys: the first, one in the middle, the last."""
+    for entries in ((0,), (300,), (518,), (0, 255, 256, 518)):
+        c = _attn_case([8_300], [70], 1, 1, D, 16, BF, 16)
+        c["table"][0, list(entries)] = -1
+        _attn_close(_run_attn(c, max_new=70, max_len=8_300), c)

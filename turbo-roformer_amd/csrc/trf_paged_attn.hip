@@ -543,9 +543,10 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && QT == 1 ? 3 : 2) void k_pag
   for (int st = 0; st < min(kFirst + M::kAhead, n_stages); ++st) stage(st, page_of(st));
   int next = page_of(kFirst + M::kAhead);
 
-  // entries that are no pages: then every unit looks its groups up
+  // entries of these stages' keys that are no pages: then every unit looks its groups up
   bool bad = false;
-  const int e1 = min(((t.hi + 15) / 16 + (1 << g.gpp_shift) - 1) >> g.gpp_shift, g.a.max_pages);
+  const int last = min(int64_t(t.hi), int64_t(s1) * M::kStageKeys);
+  const int e1 = min(((last + 15) / 16 + (1 << g.gpp_shift) - 1) >> g.gpp_shift, g.a.max_pages);
   for (int e = (first_key >> g.page_shift) + lane; e < e1; e += 64) bad |= uint32_t(table[e]) >= uint32_t(g.n_pages);
   const bool any_bad = __any(bad);
 
