@@ -420,7 +420,8 @@ size_t trf_paged_attention_workspace_bytes(int32_t heads, int32_t dtype, int32_t
  * those with j > p - window; keys whose table entry is no page count as unseen.  A row that sees none is zero, and so
  * is one whose scores are all minus infinity.  What K and V hold in places that a row does not see, infinities and NaN
  * included, does not change it.  gate [n_rows][heads] fp32 is optional (NULL: 1).  Rows of O behind the last request
- * are left as they are.
+ * are left as they are.  O may be q itself if its rows are heads * head_dim elements apart; it must not overlap it
+ * otherwise.
  * max_new and max_len are the caller's bounds on the rows and the length of a request, from which the launch is
  * chosen: rows past max_new may be left out, max_len bounds nothing but speed.  n_rows * heads is below 2^31, and
  * (n_rows * heads / kv_heads / 32 + n_requests) * kv_heads below 2^24.  P is rounded to the dtype for P V,

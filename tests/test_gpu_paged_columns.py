@@ -14,7 +14,7 @@ import torch
 from oracle import paged
 from turbo_roformer_amd import _hip
 
-from .test_gpu_paged import BF, HF, _attn_case, _attn_close, _run_attn, _say
+from .test_gpu_paged import BF, DEV, HF, _attn_case, _attn_close, _run_attn, _say
 from .test_gpu_paged_nan import _set_rows, _slot
 
 pytestmark = pytest.mark.gpu
@@ -100,3 +100,16 @@ def test_entries_that_are_no_pages_in_some_of_the_parts(hip, D):
         c = _attn_case([8_300], [70], 1, 1, D, 16, BF, 16)
         c["table"][0, list(entries)] = -1
         _attn_close(_run_attn(c, max_new=70, max_len=8_300), c)
+
+
+@pytest.mark.parametrize("D", (64, 128))
+@pytest.mark.parametrize("lens,new,heads", [([90, 40], [3, 1], 4), ([3000], [1], 8), ([500, 90], [200, 90], 1), ([2000], [60], 1),
+                                            ([700], [400], 4)])
+def test_attention_in_place_of_its_queries(hip, D, lens, new, heads):
+    c = _attn_case(lens, new, heads, 1, D, 16, BF, 18, padding=2)
+    d = {k: v.to(DEV) for k, v in c.items()}
+    n = c["q"].shape[0]
+    want = torch.cat((_run_attn(c, max_new=max(new))[:-2], c["q"][-2:]))
+    _hip.paged_attention(**d, O=d["q"].view(n, heads * D), max_new=max(new))
+    torch.cuda.synchronize()
+    assert torch.equal(d["q"].cpu(), want)

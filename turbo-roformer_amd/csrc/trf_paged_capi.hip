@@ -74,6 +74,15 @@ int check_rows(const char* name, const void* p, int64_t stride, int32_t heads, i
   return TRF_OK;
 }
 
+// Rows out [n_rows][row] beside rows q: in the same place, if both lie alike, or apart.
+int check_rows_out(const char* name, const void* out, const void* q, int64_t q_stride, int32_t n_rows, int64_t row) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(q), b = reinterpret_cast<uintptr_t>(out);
+  const bool apart = b + uintptr_t(n_rows * row * 2) <= a || a + uintptr_t(((n_rows - 1) * q_stride + row) * 2) <= b;
+  if (!apart && !(a == b && q_stride == row))
+    return set_error(TRF_ERR_ARG, "%s must not overlap q, unless it is q with rows of heads * head_dim elements", name);
+  return TRF_OK;
+}
+
 int check_state(const int32_t* state, const int32_t* state_out, int32_t n_requests) {
   TRF_REQUIRE_AT(state, "state", 4);
   TRF_REQUIRE_AT(state_out, "state_out", 4);
@@ -161,11 +170,7 @@ int trf_paged_append(const uint16_t* q, int64_t q_stride, int32_t heads, const u
   if (q) {
     TRF_TRY(check_rows("q", q, q_stride, heads, head_dim));
     TRF_REQUIRE_AT(q_out, "q_out", 16);
-    const int64_t row = int64_t(heads) * head_dim;
-    const uintptr_t a = reinterpret_cast<uintptr_t>(q), b = reinterpret_cast<uintptr_t>(q_out);
-    const bool apart = b + uintptr_t(n_rows * row * 2) <= a || a + uintptr_t(((n_rows - 1) * q_stride + row) * 2) <= b;
-    if (!apart && !(a == b && q_stride == row))
-      return set_error(TRF_ERR_ARG, "q_out must not overlap q, unless it is q with rows of heads * head_dim elements");
+    TRF_TRY(check_rows_out("q_out", q_out, q, q_stride, n_rows, int64_t(heads) * head_dim));
   }
   trf::launch_paged_append(s, q, q_stride, heads, k, k_stride, v, v_stride, K, V, slots, positions, n_rows, rope, rope_len,
                            q_out, as_hip(stream));
@@ -227,6 +232,7 @@ int trf_paged_attention(const uint16_t* q, int64_t q_stride, int32_t heads, cons
   TRF_REQUIRE_AT(lens, "lens", 4);
   if (gate) TRF_REQUIRE_AT(gate, "gate", 4);
   TRF_REQUIRE_AT(O, "O", 16);
+  TRF_TRY(check_rows_out("O", O, q, q_stride, n_rows, int64_t(heads) * head_dim));
   a.causal = causal;
   a.window = window;
   const size_t need = trf::paged_attention_workspace(s, a);
