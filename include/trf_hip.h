@@ -399,7 +399,8 @@ int trf_page_release(const int32_t* state, const uint8_t* done, int32_t n_reques
  * (feature pairs 2i, 2i + 1; rope = [2][rope_len][head_dim / 2] fp32, cos then sin, read at positions[row]; fp32
  * arithmetic, one rounding).  q (optional, [n_rows][heads][head_dim]) is rotated likewise into q_out (rows of
  * heads * head_dim), which may be q itself if its rows are that far apart.  Row strides are in elements, multiples
- * of 8; a row's heads are contiguous; n_rows * (heads + kv_heads) is below 2^28.  rope = NULL: no rotation (positions
+ * of 8; a row's heads are contiguous; n_rows, up to the next multiple of 16, times
+ * heads + kv_heads is below 2^28.  rope = NULL: no rotation (positions
  * are not read).  A row whose slot is not one of the cache, or whose position is not one of the table, is left out:
  * nothing of it is written.  Of two rows with the same slot either may be the one that is kept, value by value. */
 int trf_paged_append(const uint16_t* q, int64_t q_stride, int32_t heads, const uint16_t* k, int64_t k_stride,

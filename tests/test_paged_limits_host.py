@@ -6,7 +6,7 @@ import pytest
 
 from turbo_roformer_amd import _hip
 
-from .test_paged_host import _attend, _p
+from .test_paged_host import _append, _attend, _p
 
 
 @pytest.fixture(scope="module")
@@ -25,3 +25,11 @@ def test_attention_refuses_an_output_across_its_queries(lib, at, stride):
     """Eight rows of 512 elements at 2^16: another workgroup's rows of O would be read as q."""
     assert _attend(lib, q=_p(1 << 16), qs=stride, O=_p(at)) == 1
     assert b"O must not overlap q" in lib.trf_last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(rows=(1 << 24) - 1, heads=8, kv=8, qs=1024, ks=1024, vs=1024, q=_p(1 << 16), q_out=_p(1 << 45)),
+                                dict(rows=(1 << 27) - 1, q=None, kv=2, ks=256, vs=256), dict(rows=(1 << 28) - 1, q=None, kv=1, ks=128, vs=128)])
+def test_append_refuses_more_workgroups_than_a_launch_numbers(lib, kw):
+    """256 threads for each 16 rows and head, all of them in 32 bits."""
+    assert _append(lib, dim=128, **kw) == 1
+    assert b"n_rows" in lib.trf_last_error()

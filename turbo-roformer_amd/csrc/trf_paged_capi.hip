@@ -154,8 +154,10 @@ int trf_paged_append(const uint16_t* q, int64_t q_stride, int32_t heads, const u
   trf::PagedShape s{};
   TRF_TRY(check_cache(dtype, n_pages, page_size, kv_heads, head_dim, s));
   if (q && (heads < 1 || heads > 65535)) return set_error(TRF_ERR_ARG, "heads must be 1..65535, got %d", heads);
-  if (n_rows < 0 || int64_t(n_rows) * (kv_heads + (q ? heads : 0)) >= int64_t(1) << 28)
-    return set_error(TRF_ERR_ARG, "n_rows must be >= 0 and n_rows * (heads + kv_heads) below 2^28, got %d", n_rows);
+  // a workgroup of 256 threads per 16 rows and head, and 32 bits for a launch's threads
+  if (n_rows < 0 || (int64_t(n_rows) + 15) / 16 * (kv_heads + (q ? heads : 0)) >= int64_t(1) << 24)
+    return set_error(TRF_ERR_ARG, "n_rows must be >= 0 and n_rows, up to the next 16, * (heads + kv_heads) below 2^28, got %d",
+                     n_rows);
   if (rope && rope_len < 1) return set_error(TRF_ERR_ARG, "rope_len must be >= 1, got %d", rope_len);
   if (n_rows == 0) return TRF_OK;
   TRF_TRY(check_rows("k", k, k_stride, kv_heads, head_dim));
