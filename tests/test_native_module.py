@@ -77,3 +77,30 @@ def test_the_library_builds_without_python():
     csrc = Path(__file__).resolve().parents[1] / "turbo-roformer_amd" / "csrc"
     plan = subprocess.run(["make", "-n", "-B", "-C", str(csrc), "PYTHON=/no/such/python"], capture_output=True, text=True, check=True)
     assert "libtrf_hip.so" in plan.stdout and "trf_python.cpp" not in plan.stdout
+
+
+def test_a_tensor_without_an_address_raises(tmp_path):
+    """torch.vmap's: in a process of its own, which an exception thrown without the interpreter's lock would end."""
+    script = tmp_path / "vmapped.py"
+    script.write_text(f"""
+import sys
+sys.path.insert(0, {str(Path(_hip.__file__).resolve().parents[1])!r})
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from turbo_roformer_amd import _hip
+native = _hip.bind_native(_hip.open_library())
+with FakeTensorMode():
+    ints = lambda *shape: torch.empty(*shape, dtype=torch.int32, device="cuda:0")
+    pool, state, table = ints(8), ints(4), ints(2, 4)
+
+    def release(done):
+        try:
+            native.page_release(0, 0, state, done, pool, table, 16, state)
+        except RuntimeError:
+            print("raised")
+        return done
+
+    torch.vmap(release)(torch.empty(3, 2, dtype=torch.bool, device="cuda:0"))
+""")
+    run = subprocess.run([sys.executable, str(script)], capture_output=True, text=True, timeout=120)
+    assert run.returncode == 0 and run.stdout == "raised\n", run

@@ -139,12 +139,13 @@ PyObject* call(PyObject* const* a, Py_ssize_t got, Py_ssize_t n, F f) {
   return nullptr;
 }
 
-// f() without the interpreter's lock.
-template <class F>
-int unlocked(F f) {
+// f(a...) without the interpreter's lock.  The arguments are formed with it: asking some tensors for their address throws,
+// and the C functions do not.
+template <class F, class... A>
+int unlocked(F* f, A... a) {
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  rc = f();
+  rc = f(a...);
   Py_END_ALLOW_THREADS
   return rc;
 }
@@ -166,10 +167,8 @@ PyObject* page_plan(PyObject*, PyObject* const* a, Py_ssize_t n) {
     need(slots, "slots", at::kInt, {rows});
     int32_t* positions = ints(x, "positions", {rows});
     const int32_t longest = n == 12 ? x.number32("max_length") : int32_t(std::min<int64_t>(int64_t(max_pages) * page_size, INT32_MAX));
-    return unlocked([&] {
-      return page_plan_fn(address<int32_t>(&state), address<int32_t>(&n_new), R, rows, address<int32_t>(&pool), pages, page_size,
-                          address<int32_t>(&table), max_pages, longest, out, starts, address<int32_t>(&slots), positions, stream);
-    });
+    return unlocked(page_plan_fn, address<int32_t>(&state), address<int32_t>(&n_new), R, rows, address<int32_t>(&pool), pages,
+                    page_size, address<int32_t>(&table), max_pages, longest, out, starts, address<int32_t>(&slots), positions, stream);
   });
 }
 
@@ -183,10 +182,8 @@ PyObject* page_release(PyObject*, PyObject* const* a, Py_ssize_t n) {
     need(pool, "pool", at::kInt, {pages});
     need(table, "table", at::kInt, {R, max_pages});
     int32_t* out = ints(x, "state_out", {2 + int64_t(R)});
-    return unlocked([&] {
-      return page_release_fn(address<int32_t>(&state), address<uint8_t>(&done), R, address<int32_t>(&pool), pages, page_size,
-                             address<int32_t>(&table), max_pages, out, stream);
-    });
+    return unlocked(page_release_fn, address<int32_t>(&state), address<uint8_t>(&done), R, address<int32_t>(&pool), pages, page_size,
+                    address<int32_t>(&table), max_pages, out, stream);
   });
 }
 
@@ -213,11 +210,9 @@ PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (!q_out) throw std::invalid_argument("q needs a q_out");
       need(*q_out, "q_out", c.type, {rows, heads, c.dim});
     }
-    return unlocked([&] {
-      return paged_append_fn(address<uint16_t>(q), qs, heads, address<uint16_t>(&k), ks, address<uint16_t>(&v), vs, c.code, rows,
-                             slots, address<int32_t>(positions), address<float>(rope), P, c.K, c.V, c.pages, c.page_size, c.heads,
-                             c.dim, address<uint16_t>(q_out), stream);
-    });
+    return unlocked(paged_append_fn, address<uint16_t>(q), qs, heads, address<uint16_t>(&k), ks, address<uint16_t>(&v), vs, c.code,
+                    rows, slots, address<int32_t>(positions), address<float>(rope), P, c.K, c.V, c.pages, c.page_size, c.heads, c.dim,
+                    address<uint16_t>(q_out), stream);
   });
 }
 
@@ -245,11 +240,9 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int32_t max_len = no_len ? (x.next++, INT32_MAX) : x.number32("max_len");
     const at::Tensor* ws = x.tensor("ws", true);
     if (ws) need(*ws, "ws", at::kByte, {ws->numel()});
-    return unlocked([&] {
-      return paged_attention_fn(address<uint16_t>(&q), qs, heads, c.K, c.V, c.code, c.pages, c.page_size, c.heads, c.dim,
-                                address<int32_t>(&table), max_pages, starts, lens, R, rows, max_new, max_len, scale, causal, window,
-                                address<float>(gate), address<uint16_t>(&O), address<void>(ws), ws ? size_t(ws->numel()) : 0, stream);
-    });
+    return unlocked(paged_attention_fn, address<uint16_t>(&q), qs, heads, c.K, c.V, c.code, c.pages, c.page_size, c.heads, c.dim,
+                    address<int32_t>(&table), max_pages, starts, lens, R, rows, max_new, max_len, scale, causal, window,
+                    address<float>(gate), address<uint16_t>(&O), address<void>(ws), ws ? size_t(ws->numel()) : 0, stream);
   });
 }
 
