@@ -54,6 +54,18 @@ def test_a_tail_of_small_weights_is_kept(hip, D, rows, heads):
     assert float((got - want).abs().max()) <= tol, (float(got.min()), float(got.max()), want, tol)
 
 
+@pytest.mark.parametrize("D", (64, 128))
+@pytest.mark.parametrize("rows,heads", [(1, 1), (40, 1), (300, 4)])
+def test_the_weights_of_a_tail_add_to_one(hip, D, rows, heads):
+    """The sum that divides is that of the rounded weights that are applied, subnormal ones too: ones come out as ones (P.V
+    and the sum differ by 2^-24 of each of a few thousand additions, and one's half step is 2^-12 below it)."""
+    n = 131_072
+    k, q = torch.zeros(n, D, dtype=HF), torch.zeros(D, dtype=HF)
+    k[0, 0], q[0] = 1.0, 18.03125
+    got = _shared_pages(k, torch.ones(n, D, dtype=HF), 172 if rows < 300 else 31, rows, heads, q, HF)
+    assert bool((got == 1).all()), (float(got.min()), float(got.max()))
+
+
 @pytest.mark.parametrize("dtype", (BF, HF))
 @pytest.mark.parametrize("rows,heads", [(1, 1), (40, 1), (300, 4)])
 def test_scores_of_millions(hip, dtype, rows, heads):
