@@ -331,9 +331,9 @@ __device__ __forceinline__ void split_range(const Args& g, const Tile& t, int wi
 // A workgroup has one tile of 32 columns; its four waves take every fourth 32-key tile, K and V^T operands straight
 // from the cache into registers (each byte of the cache is used once, so LDS would only pass it on), and join their sums
 // in LDS at the end.  Bound by HBM, or by latency for short caches: single rows of 5 sequences of 100,000 to 131,000 keys,
-// 32 and 8 heads of 128, 398-410 us with the join (5.7-5.9 TB/s; one tile at a time 408 + 20, as it came first 2475); one row of 62
-// sequences of 600 to 1701 keys, 8 heads of 64, 31.6 us (4.6 TB/s: two workgroups a CU of unequal lengths); one row of 17
-// keys 5.1 us.  Head dim 128 runs one wave a SIMD, with all its registers: at two, with one tile each, 443 us.
+// 32 and 8 heads of 128, 407-425 us by host with the join (5.5-5.7 TB/s; one tile at a time 408 + 20, as it came first 2475);
+// one row of 62 sequences of 600 to 1701 keys, 8 heads of 64, 32 us (4.6 TB/s: two workgroups a CU of unequal lengths); one
+// row of 17 keys 5.1 us.  Head dim 128 runs one wave a SIMD, with all its registers: at two, with one tile each, 443 us.
 template <int D, bool F16>
 __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void k_paged_attn_few(Args g) {
   constexpr int KS = D / 16, DT = D / 32;
@@ -479,11 +479,12 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void k_paged_attn_few
 // take turns on the two column tiles, and each K and V operand read from LDS feeds two products.  Raising the maximum,
 // masks and infinities leave that path (rare).
 //
-// Bound by the matrix pipe beside the softmax's vector work (about 50 instructions and 16 exponentials a step, for 12
-// (D = 64) or 20 MFMAs, 4 of them small), and by the clock that the power limit leaves, 1.9-2.1 GHz.  Measured: 62 sequences of 1701 rows
-// over 1701 keys, 8 heads of 64, 412-452 us by host (810-890 TFLOP/s; a large library matrix product reaches 1190); 9
-// sequences of 300 to 600 rows over 2400 to 5800 keys, 32 and 8 heads of 128, 278-292 us (830-870 TFLOP/s: 1104 workgroups in
-// 2.2 rounds of 512); 8 of 700 rows over 6000 keys 526 us (985 TFLOP/s).  Steps on the way (us for the first and the
+// Bound by issue and by waits, about alike, beside a matrix pipe that is busy 44% of the cycles at 1.9-2.1 GHz: about 50
+// vector instructions and 16 exponentials a step, for 12 (D = 64) or 20 MFMAs, 4 of them small; of a wave's cycles
+// 47% (40% at D = 128) issue, 27% (35%) wait for their turn, 26% (24%) for loads and the stages' barriers.  Measured: 62 sequences of 1701 rows
+// over 1701 keys, 8 heads of 64, 432-444 us by host (830-850 TFLOP/s; a large library matrix product reaches 1190); 9
+// sequences of 300 to 600 rows over 2400 to 5800 keys, 32 and 8 heads of 128, 280-288 us (840-870 TFLOP/s: 1104 workgroups in
+// 2.2 rounds of 512); 8 of 700 rows over 6000 keys 524 us (990 TFLOP/s).  Steps on the way (us for the first and the
 // second): K and V through LDS 566 and 371, three steps at once 521 and 344, two column tiles a wave and a loop without
 // edges 486 and 331.
 template <int D, int QT>
