@@ -485,8 +485,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 ? 2 : 1) void k_paged_attn_few
 // sequences of 1701 rows over 1701 keys, 8 heads of 64, 432-444 us by host (830-850 TFLOP/s; a large library matrix product
 // reaches 1190); 9 sequences of 300 to 600 rows over 2400 to 5800 keys, 32 and 8 heads of 128, 280-288 us (840-870
 // TFLOP/s: 1104 workgroups in 2.2 rounds of 512); 8 of 700 rows over 6000 keys 524 us (990 TFLOP/s).  Steps on the way (us
-// for the first and the second: K and V through LDS 566 and 371, three steps at once 521 and 344, two column tiles a wave and a loop without
-// edges 486 and 331.
+// for the first and the second): K and V through LDS 566 and 371, three steps at once 521 and 344, two column tiles a wave
+// and a loop without edges 486 and 331.
 template <int D, int QT>
 struct Many {
   static constexpr int kStageKeys = D == 64 ? 64 : 32, kUnits = kStageKeys / 32;  // keys and units of a stage
